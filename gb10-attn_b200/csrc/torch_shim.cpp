@@ -583,6 +583,156 @@ std::tuple<torch::Tensor, torch::Tensor> merge_states(torch::Tensor outs, torch:
   return {out, lse};
 }
 
+// The layers' pool tensors as pointer arrays; contiguous and alike.
+struct PoolLayers {
+  std::vector<void*> k, v;
+};
+static PoolLayers pool_layers(const std::vector<torch::Tensor>& k_layers,
+                              const std::vector<torch::Tensor>& v_layers, const char* op) {
+  TORCH_CHECK(!k_layers.empty() && k_layers.size() == v_layers.size(),
+              op, ": need one K and one V tensor per layer");
+  const torch::Tensor& k0 = k_layers[0];
+  TORCH_CHECK(k0.is_cuda() && k0.dim() == 4, op, ": pool tensors must be CUDA [NB, BS, H, D]");
+  PoolLayers p;
+  for (size_t l = 0; l < k_layers.size(); ++l) {
+    for (const torch::Tensor* t : {&k_layers[l], &v_layers[l]})
+      TORCH_CHECK(t->is_contiguous() && t->sizes() == k0.sizes() &&
+                      t->scalar_type() == k0.scalar_type() && t->device() == k0.device(),
+                  op, ": pool tensors must be contiguous and alike");
+    p.k.push_back(k_layers[l].data_ptr());
+    p.v.push_back(v_layers[l].data_ptr());
+  }
+  return p;
+}
+
+// Page copies for every layer (pa_copy_blocks): block src_blocks[i] to
+// dst_blocks[i], its first num_rows[i] token rows (an empty tensor: the whole
+// page).  The pool tensors are written in place.
+void copy_blocks(std::vector<torch::Tensor> k_layers, std::vector<torch::Tensor> v_layers,
+                 torch::Tensor src_blocks, torch::Tensor dst_blocks, torch::Tensor num_rows) {
+  const char* op = "copy_blocks";
+  const PoolLayers pl = pool_layers(k_layers, v_layers, op);
+  const torch::Tensor& k0 = k_layers[0];
+  const c10::cuda::CUDAGuard guard(k0.device());
+  torch::Tensor src = src_blocks.to(k0.device(), torch::kInt32).contiguous();
+  torch::Tensor dst = dst_blocks.to(k0.device(), torch::kInt32).contiguous();
+  torch::Tensor rows;
+  TORCH_CHECK(src.dim() == 1 && dst.sizes() == src.sizes(),
+              op, ": src_blocks and dst_blocks must be [n]");
+  if (num_rows.defined() && num_rows.numel()) {
+    rows = num_rows.to(k0.device(), torch::kInt32).contiguous();
+    TORCH_CHECK(rows.sizes() == src.sizes(), op, ": num_rows must be [n] or empty");
+  }
+  check_status(pa_copy_blocks(pl.k.data(), pl.v.data(), pool_dtype(k0, op), src.data_ptr<int32_t>(),
+                              dst.data_ptr<int32_t>(),
+                              rows.defined() ? rows.data_ptr<int32_t>() : nullptr, src.numel(),
+                              (int64_t)pl.k.size(), k0.size(2), k0.size(3), k0.size(1), k0.size(0),
+                              nullptr, stream_ptr()),
+               op);
+}
+
+// New block tables with every entry inside the pool replaced by its block_map
+// entry ([num_blocks]).
+torch::Tensor remap_block_tables(torch::Tensor block_tables, torch::Tensor block_map) {
+  const char* op = "remap_block_tables";
+  TORCH_CHECK(block_tables.is_cuda(), "block_tables must be on CUDA");
+  const c10::cuda::CUDAGuard guard(block_tables.device());
+  torch::Tensor bt = block_tables.to(torch::kInt32).contiguous();
+  torch::Tensor map = block_map.to(bt.device(), torch::kInt32).contiguous();
+  TORCH_CHECK(map.dim() == 1, op, ": block_map must be [num_blocks]");
+  torch::Tensor out = torch::empty_like(bt);
+  check_status(pa_remap_block_tables(out.data_ptr<int32_t>(), bt.data_ptr<int32_t>(),
+                                     map.data_ptr<int32_t>(), bt.numel(), map.numel(),
+                                     stream_ptr()),
+               op);
+  return out;
+}
+
+// Norm and rotation of q and k, q out, k and v to their pool rows
+// (pa_qk_norm_rope_append).  q [T, H, D], k, v [T, HKV, D]; empty weights: no
+// norm; cos_sin [max_pos, rot_dim] fp32; seq_ids [T] or empty (token t is of
+// sequence t); k_scale / v_scale [HKV] for FP8 pools or empty.
+torch::Tensor qk_norm_rope_append(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                  torch::Tensor q_weight, torch::Tensor k_weight, double eps,
+                                  torch::Tensor cos_sin, bool interleaved, torch::Tensor positions,
+                                  torch::Tensor seq_ids, torch::Tensor k_cache,
+                                  torch::Tensor v_cache, torch::Tensor block_tables,
+                                  torch::Tensor k_scale, torch::Tensor v_scale) {
+  const char* op = "qk_norm_rope_append";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, op, ": q must be a CUDA [T, H, D] tensor");
+  int io;
+  switch (q.scalar_type()) {
+    case torch::kFloat: io = PA_DTYPE_F32; break;
+    case torch::kHalf: io = PA_DTYPE_F16; break;
+    case torch::kBFloat16: io = PA_DTYPE_BF16; break;
+    default: TORCH_CHECK(false, op, ": q must be float32, float16 or bfloat16");
+  }
+  TORCH_CHECK(k_cache.is_cuda() && k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
+                  v_cache.scalar_type() == k_cache.scalar_type() && k_cache.device() == q.device() &&
+                  v_cache.device() == q.device(),
+              op, ": k_cache, v_cache must be alike CUDA [NB, BS, HKV, D] tensors");
+  TORCH_CHECK(k_cache.is_contiguous() && v_cache.is_contiguous(),
+              op, ": the pool is written in place, so it must be contiguous");
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  const int64_t NB = k_cache.size(0), BS = k_cache.size(1), HKV = k_cache.size(2);
+  TORCH_CHECK(k_cache.size(3) == D, op, ": k_cache head_dim must match q");
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && k.size(0) == T && k.size(1) == HKV &&
+                  k.size(2) == D && k.scalar_type() == q.scalar_type() &&
+                  v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                  v.device() == q.device(),
+              op, ": k, v must be [T, HKV, D] of q's type on its device");
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.scalar_type() == torch::kFloat,
+              op, ": cos_sin must be float32 [max_positions, rot_dim]");
+  const c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor qs = q.stride(2) == 1 ? q : q.contiguous();
+  torch::Tensor ks = k.stride(2) == 1 ? k : k.contiguous();
+  torch::Tensor vs = v.stride(2) == 1 ? v : v.contiguous();
+  torch::Tensor cs = cos_sin.to(q.device()).contiguous();
+  torch::Tensor pos = positions.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor bt = block_tables.to(q.device(), torch::kInt32).contiguous();
+  TORCH_CHECK(pos.numel() == T && bt.dim() == 2, op, ": positions [T] and block_tables [B, MB] needed");
+  torch::Tensor ids;
+  if (seq_ids.defined() && seq_ids.numel()) {
+    ids = seq_ids.to(q.device(), torch::kInt32).contiguous();
+    TORCH_CHECK(ids.numel() == T, op, ": seq_ids must be [T] or empty");
+  } else {
+    TORCH_CHECK(T <= bt.size(0), op, ": without seq_ids, block_tables needs a row per token");
+  }
+  torch::Tensor w[2];
+  for (int i = 0; i < 2; ++i) {
+    const torch::Tensor& src = i ? k_weight : q_weight;
+    if (!src.defined() || !src.numel()) continue;
+    TORCH_CHECK(src.numel() == D, op, ": weights must be [D] or empty");
+    w[i] = src.to(q.device()).contiguous();
+  }
+  // one type for both weights: q's, or fp32
+  bool w_f32 = false;
+  for (const torch::Tensor& t : w) w_f32 |= t.defined() && t.scalar_type() != q.scalar_type();
+  for (torch::Tensor& t : w)
+    if (t.defined() && w_f32) t = t.to(torch::kFloat);
+  torch::Tensor sc[2];
+  for (int i = 0; i < 2; ++i) {
+    const torch::Tensor& src = i ? v_scale : k_scale;
+    if (!src.defined() || !src.numel()) continue;
+    sc[i] = src.to(q.device(), torch::kFloat).contiguous();
+    TORCH_CHECK(sc[i].numel() == HKV, op, ": scales must be [HKV] or empty");
+  }
+  torch::Tensor out = torch::empty({T, H, D}, q.options());
+  check_status(pa_qk_norm_rope_append(
+                   out.data_ptr(), qs.data_ptr(), qs.stride(0), qs.stride(1), ks.data_ptr(),
+                   ks.stride(0), ks.stride(1), vs.data_ptr(), vs.stride(0), vs.stride(1), io,
+                   w[0].defined() ? w[0].data_ptr() : nullptr,
+                   w[1].defined() ? w[1].data_ptr() : nullptr, w_f32 ? PA_DTYPE_F32 : io, eps,
+                   cs.data_ptr<float>(), cs.size(0), cs.size(1), interleaved ? 1 : 0,
+                   pos.data_ptr<int32_t>(), ids.defined() ? ids.data_ptr<int32_t>() : nullptr, T,
+                   k_cache.data_ptr(), v_cache.data_ptr(), pool_dtype(k_cache, op),
+                   sc[0].defined() ? sc[0].data_ptr<float>() : nullptr,
+                   sc[1].defined() ? sc[1].data_ptr<float>() : nullptr, bt.data_ptr<int32_t>(),
+                   bt.size(0), H, HKV, D, BS, NB, bt.size(1), nullptr, stream_ptr()),
+               op);
+  return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 paged attention: the gb10-attn operator API over libpa_b200.so";
   m.def("paged_attention", &paged_attention);
@@ -601,4 +751,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_v3_fp8", &paged_attention_v3_fp8);
   m.def("validate_block_tables", &validate_block_tables);
   m.def("merge_states", &merge_states);
+  m.def("qk_norm_rope_append", &qk_norm_rope_append);
+  m.def("copy_blocks", &copy_blocks);
+  m.def("remap_block_tables", &remap_block_tables);
 }

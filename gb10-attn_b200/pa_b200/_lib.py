@@ -90,6 +90,11 @@ SIGNATURES = {
                      [_P, _P, _P, _P]),
     "pa_decode_layer_step": (_I, [_P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P] + [_I64] * 7 +
                              [_D, _I64, _P, _SZ, _P, _P]),
+    "pa_copy_blocks": (_I, [_P, _P, _I, _P, _P, _P] + [_I64] * 6 + [_P, _P]),
+    "pa_remap_block_tables": (_I, [_P, _P, _P, _I64, _I64, _P]),
+    "pa_qk_norm_rope_append": (_I, [_P] + [_P, _I64, _I64] * 3 + [_I, _P, _P, _I, _D, _P, _I64, _I64,
+                                                                  _I, _P, _P, _I64, _P, _P, _I, _P,
+                                                                  _P, _P] + [_I64] * 7 + [_P, _P]),
     "pa_validate_block_tables": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _P]),
 }
 

@@ -156,6 +156,7 @@ class TorchBlockAllocator:
                                        device=self.device)
             self.v_scales = torch.ones_like(self.k_scales)
         self._free = list(range(kv_cfg.num_blocks - 1, -1, -1))
+        self._shared: dict[int, int] = {}  # block -> holders beyond the first
 
     def set_scales(self, k_scales, v_scales) -> None:
         """FP8 pools: the [n_layer, n_kv_head] quantisation scales used by
@@ -186,7 +187,95 @@ class TorchBlockAllocator:
         return Allocation(blocks, len(ids), ids)
 
     def free(self, block_ids) -> None:
-        self._free.extend(reversed(list(block_ids)))
+        """Give up one hold on each block; a block that forks share goes back
+        to the pool with its last holder."""
+        for b in reversed(list(block_ids)):
+            left = self._shared.get(b, 0)
+            if left == 0:
+                self._free.append(b)
+            elif left == 1:
+                del self._shared[b]
+            else:
+                self._shared[b] = left - 1
+
+    def holders(self, block_id: int) -> int:
+        """Allocations that hold a block which is in use."""
+        return 1 + self._shared.get(block_id, 0)
+
+    def fork(self, allocation: Allocation, n: int = 1, num_tokens: int | None = None
+             ) -> list[Allocation]:
+        """n sequences that start with the first num_tokens (default: all)
+        tokens of ``allocation``.  Full pages are shared; the page in which the
+        tokens end, if it is part-filled, is copied for every fork (one launch,
+        every layer), so no two sequences ever write the same page."""
+        t = allocation.num_tokens if num_tokens is None else int(num_tokens)
+        if not 0 <= t <= allocation.num_tokens:
+            raise ValueError(f"fork at {t} of {allocation.num_tokens} tokens")
+        full, rows = divmod(t, self.kv_cfg.block_size)
+        if rows and n > len(self._free):
+            raise MemoryError(f"KV pool exhausted: need {n} blocks, {len(self._free)} free")
+        shared = allocation.block_ids[:full]
+        if n > 0:
+            for b in shared:
+                self._shared[b] = self._shared.get(b, 0) + n
+        last = [self._free.pop() for _ in range(n)] if rows else []
+        if last:
+            self.copy_blocks([allocation.block_ids[full]] * n, last, [rows] * n)
+        return [Allocation(shared + last[i:i + 1], t, list(allocation.token_ids[:t]))
+                for i in range(n)]
+
+    def extend(self, allocation: Allocation, token_ids) -> None:
+        """Room for further tokens of a sequence (pages are taken as needed)."""
+        ids = list(token_ids)
+        need = self.blocks_for(allocation.num_tokens + len(ids)) - len(allocation.block_ids)
+        if need > len(self._free):
+            raise MemoryError(f"KV pool exhausted: need {need} blocks, {len(self._free)} free")
+        allocation.block_ids.extend(self._free.pop() for _ in range(need))
+        allocation.num_tokens += len(ids)
+        allocation.token_ids.extend(ids)
+
+    def copy_blocks(self, src, dst, num_rows=None) -> None:
+        """Copy pages src[i] -> dst[i] in every layer (their first num_rows[i]
+        token rows if given), one launch."""
+        from . import ops
+
+        def dev(x):
+            if isinstance(x, torch.Tensor):
+                return x.to(device=self.device, dtype=torch.int32)
+            return torch.tensor(list(x), dtype=torch.int32).to(self.device)
+
+        n_layer = self.model_cfg.n_layer
+        ks = [self.pool[layer, 0] for layer in range(n_layer)]
+        vs = [self.pool[layer, 1] for layer in range(n_layer)]
+        ops.copy_blocks(ks, vs, dev(src), dev(dst),
+                        torch.empty(0) if num_rows is None else dev(num_rows))
+
+    def compact(self, allocations) -> torch.Tensor | None:
+        """Move the pages in use to the lowest block ids, so that the blocks
+        from ``kv_cfg.num_blocks - num_free_blocks`` on are free.  ``allocations``
+        holds every live allocation; their block ids are rewritten.  Returns
+        the [num_blocks] int32 map old id -> new id on the device (for
+        ``ops.remap_block_tables`` on tables that are there already), or None
+        if nothing moved."""
+        used = self.kv_cfg.num_blocks - len(self._free)
+        free = set(self._free)
+        src = [b for b in range(used, self.kv_cfg.num_blocks) if b not in free]
+        dst = sorted(b for b in free if b < used)
+        if not src:
+            return None
+        held = {b for a in allocations for b in a.block_ids}
+        lost = [b for b in src if b not in held]
+        if lost:
+            raise ValueError(f"compact: blocks {lost[:8]} are in use by no allocation given")
+        self.copy_blocks(src, dst)
+        to = dict(zip(src, dst))
+        for a in allocations:
+            a.block_ids[:] = [to.get(b, b) for b in a.block_ids]
+        self._shared = {to.get(b, b): n for b, n in self._shared.items()}
+        self._free = list(range(self.kv_cfg.num_blocks - 1, used - 1, -1))
+        block_map = torch.arange(self.kv_cfg.num_blocks, dtype=torch.int32)
+        block_map[torch.tensor(src)] = torch.tensor(dst, dtype=torch.int32)
+        return block_map.to(self.device)
 
     def capacity_headroom(self) -> dict:
         """Free blocks and the margin of the largest single pool tensor below

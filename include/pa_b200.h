@@ -447,6 +447,71 @@ PA_API int pa_validate_block_tables(const int32_t* block_tables,
                              int64_t num_blocks, int32_t* counts,
                              void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* pages shared between sequences                                            */
+/* ------------------------------------------------------------------------ */
+/* Additions: the reference's pool gives every sequence pages of its own
+ * (hetero-serve heteroserve/kv/torch_blocks.py, un-vendored). */
+
+/* Copy pages inside the pool, every layer's K and V in one launch: for each
+ * pair i < num_pairs, the first num_rows[i] token rows (clamped to [0, BS];
+ * num_rows NULL = the whole page) of block src_blocks[i] go to the same rows of
+ * block dst_blocks[i].  k_layers / v_layers: HOST arrays of num_layers device
+ * pointers, as for pa_write_kv; src_blocks, dst_blocks, num_rows: device int32
+ * [num_pairs].  Any pool dtype.  The destinations must differ from one another
+ * and from every source (a pair whose source is its destination does nothing).
+ * A pair with a block id outside [0, num_blocks) is skipped and reported as
+ * PA_DEVERR_BLOCK_ID.  Offsets are 64-bit. */
+PA_API int pa_copy_blocks(void* const* k_layers, void* const* v_layers, int pool_dtype,
+                          const int32_t* src_blocks, const int32_t* dst_blocks,
+                          const int32_t* num_rows, int64_t num_pairs, int64_t num_layers,
+                          int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                          int64_t num_blocks, int32_t* dev_status, void* stream);
+
+/* out[i] = block_map[block_tables[i]] for entries inside [0, num_blocks);
+ * other entries are copied as they are.  block_map: device int32 [num_blocks].
+ * out may be block_tables itself. */
+PA_API int pa_remap_block_tables(int32_t* out, const int32_t* block_tables,
+                                 const int32_t* block_map, int64_t num_entries,
+                                 int64_t num_blocks, void* stream);
+
+/* From a layer's q / k / v projection to its attention, an addition (the
+ * reference's model has neither norms of q and k nor a rotation): for every
+ * token t < num_tokens and head x of q and k (D = head_dim elements, fp32
+ * arithmetic),
+ *   y = x * weight / sqrt(mean(x^2) + eps)    (q_weight / k_weight [D]; NULL:
+ *                                              y = x, no norm)
+ * and the first rot_dim elements turn in pairs, pair i by the angle whose
+ * cosine and sine are cos_sin[positions[t]][i] and [rot_dim / 2 + i]:
+ *   (a, b) -> (a cos - b sin, b cos + a sin)
+ * where pair i is elements (i, i + rot_dim / 2), or (2i, 2i + 1) if
+ * interleaved != 0.  q goes to q_out [num_tokens, num_heads, head_dim]
+ * (contiguous, io_dtype); k so treated and v as it is go to position
+ * positions[t] of sequence seq_ids[t] (NULL: token t is of sequence t, and
+ * num_tokens <= num_seqs) through its block-table row, converted as
+ * pa_write_kv_scaled does (k_scale / v_scale: [num_kv_heads] of this layer,
+ * FP8 pools only, nullable).  No two tokens may name the same pool row.
+ *
+ * q, k, v: device, io_dtype (fp32, fp16 or bf16), head_dim contiguous, the
+ * given element strides between tokens and heads (so they may be parts of one
+ * projection's output).  weight_dtype: PA_DTYPE_F32 or io_dtype.  cos_sin:
+ * device fp32 [max_positions, rot_dim].  rot_dim: even, 0 .. head_dim.
+ * head_dim in {32, 64, 128, 256}.  A token with positions[t] < 0 is padding:
+ * its q_out is zero and nothing is appended.  A position past max_positions
+ * gives NaN in q_out and no append, a sequence or position outside the block
+ * tables no append, both reported as PA_DEVERR_CONTEXT; a block id outside
+ * [0, num_blocks) no append and PA_DEVERR_BLOCK_ID. */
+PA_API int pa_qk_norm_rope_append(
+    void* q_out, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+    int64_t v_head_stride, int io_dtype, const void* q_weight, const void* k_weight,
+    int weight_dtype, double eps, const float* cos_sin, int64_t max_positions, int64_t rot_dim,
+    int interleaved, const int32_t* positions, const int32_t* seq_ids, int64_t num_tokens,
+    void* k_cache, void* v_cache, int kv_dtype, const float* k_scale, const float* v_scale,
+    const int32_t* block_tables, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t max_blocks,
+    int32_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,52 @@
+"""The entry points for sequences that share pages: what they refuse before
+they touch a device."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from pa_b200 import _lib
+
+BAD = _lib.PA_ERR_INVALID_ARGUMENT
+ONE = (ctypes.c_void_p * 1)(16)
+NONE = (ctypes.c_void_p * 1)(None)
+P = ctypes.c_void_p(16)
+
+
+@pytest.mark.parametrize("args,want", [
+    ((ONE, ONE, 17, P, P, None, 1, 1, 2, 64, 16, 8), _lib.PA_ERR_DTYPE),
+    ((ONE, ONE, 1, P, P, None, -1, 1, 2, 64, 16, 8), BAD),
+    ((ONE, ONE, 1, P, P, None, 1, 1, 0, 64, 16, 8), BAD),
+    ((ONE, ONE, 1, P, P, None, 1, 1, 2, 64, 0, 8), BAD),
+    ((ONE, ONE, 1, None, P, None, 1, 1, 2, 64, 16, 8), BAD),
+    ((ONE, ONE, 1, P, None, None, 1, 1, 2, 64, 16, 8), BAD),
+    ((None, ONE, 1, P, P, None, 1, 1, 2, 64, 16, 8), BAD),
+    ((NONE, ONE, 1, P, P, None, 1, 1, 2, 64, 16, 8), BAD),
+    ((None, None, 1, None, None, None, 0, 1, 2, 64, 16, 8), _lib.PA_OK),
+    ((None, None, 1, P, P, None, 3, 0, 2, 64, 16, 8), _lib.PA_OK),
+])
+def test_copy_blocks(args, want):
+    assert _lib.call("pa_copy_blocks", *args, None, None) == want
+
+
+def test_remap_block_tables():
+    assert _lib.call("pa_remap_block_tables", P, P, P, -1, 4, None) == BAD
+    assert _lib.call("pa_remap_block_tables", None, P, P, 1, 4, None) == BAD
+    assert _lib.call("pa_remap_block_tables", P, P, None, 1, 4, None) == BAD
+    assert _lib.call("pa_remap_block_tables", None, None, None, 0, 4, None) == _lib.PA_OK
+
+
+def _append(io=2, kv=2, T=1, seqs=1, rot=64, D=64, q=P, pos=P, cs=P, seq=P, wdt=0, H=2, BS=16):
+    return _lib.call("pa_qk_norm_rope_append", P, q, 128, 64, P, 64, 64, P, 64, 64, io, P, P, wdt, 1e-6, cs, 10, rot,
+                     0, pos, seq, T, P, P, kv, None, None, P, seqs, H, 1, D, BS, 8, 4, None, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    ({"T": -1}, BAD), ({"H": 0}, BAD), ({"BS": 0}, BAD), ({"rot": 63}, BAD), ({"rot": 66}, BAD), ({"rot": -2}, BAD),
+    ({"D": 96}, _lib.PA_ERR_HEAD_DIM), ({"io": 3}, _lib.PA_ERR_DTYPE), ({"io": 4}, _lib.PA_ERR_DTYPE),
+    ({"kv": 9}, _lib.PA_ERR_DTYPE), ({"wdt": 1}, _lib.PA_ERR_DTYPE), ({"T": 2, "seq": None}, BAD),
+    ({"q": None}, BAD), ({"pos": None}, BAD), ({"cs": None}, BAD), ({"T": 0, "q": None}, _lib.PA_OK),
+])
+def test_qk_norm_rope_append(kw, want):
+    assert _append(**kw) == want
