@@ -733,6 +733,54 @@ torch::Tensor qk_norm_rope_append(torch::Tensor q, torch::Tensor k, torch::Tenso
   return out;
 }
 
+// Decode of sequences that share prefixes (pa_paged_attention_shared): q
+// [B, H, D] of the pool's type (fp16 or bf16) gives (out of that type, lse
+// fp32 [B, H]).  Group g is sequences group_starts[g] .. group_starts[g+1]-1,
+// with the same first prefix_lens[g] tokens.
+std::tuple<torch::Tensor, torch::Tensor> paged_attention_shared(
+    torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_tables,
+    torch::Tensor context_lens, torch::Tensor group_starts, torch::Tensor prefix_lens,
+    double scale) {
+  const char* op = "paged_attention_shared";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, op, ": q must be a CUDA [B, H, D] tensor");
+  TORCH_CHECK(k_cache.is_cuda() && k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
+                  v_cache.scalar_type() == k_cache.scalar_type() && k_cache.device() == q.device() &&
+                  v_cache.device() == q.device(),
+              op, ": k_cache, v_cache must be alike CUDA [NB, BS, HKV, D] tensors");
+  TORCH_CHECK(q.scalar_type() == k_cache.scalar_type() &&
+                  (q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16),
+              op, ": q and the pool must both be float16 or both bfloat16");
+  const c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor qc = q.contiguous(), kc = k_cache.contiguous(), vc = v_cache.contiguous();
+  torch::Tensor bt = block_tables.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor ctx = context_lens.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor gs = group_starts.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor pl = prefix_lens.to(q.device(), torch::kInt32).contiguous();
+  const int64_t B = qc.size(0), H = qc.size(1), D = qc.size(2);
+  const int64_t NB = kc.size(0), BS = kc.size(1), HKV = kc.size(2), NG = pl.numel();
+  TORCH_CHECK(kc.size(3) == D, op, ": k_cache head_dim must match q");
+  TORCH_CHECK(H % HKV == 0, "n_head must be divisible by n_kv_head");
+  TORCH_CHECK(bt.dim() == 2 && bt.size(0) >= B && ctx.numel() >= B,
+              op, ": block_tables [B, MB] and context_lens [B] needed");
+  TORCH_CHECK(NG == 0 || gs.numel() == NG + 1,
+              op, ": group_starts must have one entry more than prefix_lens");
+  torch::Tensor out = torch::empty({B, H, D}, qc.options());
+  torch::Tensor lse = torch::empty({B, H}, qc.options().dtype(torch::kFloat32));
+  if (B == 0) return {out, lse};
+  const int dt = pool_dtype(kc, op);
+  size_t ws_bytes = 0;
+  check_status(pa_shared_workspace_size(B, NG, H, HKV, D, dt, &ws_bytes), op);
+  torch::Tensor ws = workspace(ws_bytes, qc);
+  check_status(pa_paged_attention_shared(
+                   out.data_ptr(), lse.data_ptr<float>(), qc.data_ptr(), dt, kc.data_ptr(),
+                   vc.data_ptr(), dt, bt.data_ptr<int32_t>(), ctx.data_ptr<int32_t>(),
+                   NG ? gs.data_ptr<int32_t>() : nullptr, NG ? pl.data_ptr<int32_t>() : nullptr, B,
+                   NG, H, HKV, D, BS, NB, bt.size(1), scale, ws.data_ptr(), ws_bytes, nullptr,
+                   stream_ptr()),
+               op);
+  return {out, lse};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 paged attention: the gb10-attn operator API over libpa_b200.so";
   m.def("paged_attention", &paged_attention);
@@ -751,6 +799,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_v3_fp8", &paged_attention_v3_fp8);
   m.def("validate_block_tables", &validate_block_tables);
   m.def("merge_states", &merge_states);
+  m.def("paged_attention_shared", &paged_attention_shared);
   m.def("qk_norm_rope_append", &qk_norm_rope_append);
   m.def("copy_blocks", &copy_blocks);
   m.def("remap_block_tables", &remap_block_tables);

@@ -28,6 +28,7 @@ PA_ERR_TOO_LARGE = 9
 PA_ERR_NO_DEVICE = 10
 PA_DEVERR_BLOCK_ID, PA_DEVERR_CONTEXT, PA_DEVERR_TIMEOUT, PA_DEVERR_MERGE = 1, 2, 4, 8
 PA_DEVERR_RANGE = 0x10
+PA_DEVERR_GROUP = 0x20
 PA_IPC_HANDLE_BYTES = 64
 
 _P = ctypes.c_void_p
@@ -95,6 +96,9 @@ SIGNATURES = {
     "pa_qk_norm_rope_append": (_I, [_P] + [_P, _I64, _I64] * 3 + [_I, _P, _P, _I, _D, _P, _I64, _I64,
                                                                   _I, _P, _P, _I64, _P, _P, _I, _P,
                                                                   _P, _P] + [_I64] * 7 + [_P, _P]),
+    "pa_shared_workspace_size": (_I, [_I64] * 5 + [_I, ctypes.POINTER(_SZ)]),
+    "pa_paged_attention_shared": (_I, [_P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P] + [_I64] * 8 +
+                                  [_D, _P, _SZ, _P, _P]),
     "pa_validate_block_tables": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _P]),
 }
 

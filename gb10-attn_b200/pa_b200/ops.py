@@ -19,6 +19,8 @@ plus ``paged_attention_v3_lse``, ``paged_attention_prefill_simt``,
 ``write_kv``, ``validate_block_tables`` and ``merge_states``, and for sequences
 that share pages::
 
+    paged_attention_shared(q, k_cache, v_cache, block_tables, context_lens,
+                           group_starts, prefix_lens, scale)     -> (out, lse)
     qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, cos_sin, interleaved,
                         positions, seq_ids, k_cache, v_cache, block_tables,
                         k_scale, v_scale)        (cos_sin from rope_table)
@@ -56,6 +58,7 @@ write_kv_scaled = _ext.write_kv_scaled
 append_kv = _ext.append_kv
 write_kv_batch = _ext.write_kv_batch
 decode_layer_step = _ext.decode_layer_step
+paged_attention_shared = _ext.paged_attention_shared
 qk_norm_rope_append = _ext.qk_norm_rope_append
 copy_blocks = _ext.copy_blocks
 remap_block_tables = _ext.remap_block_tables
@@ -65,7 +68,8 @@ __all__ = ["paged_attention", "paged_attention_v2", "paged_attention_v3",
            "paged_attention_prefill_wmma", "paged_attention_prefill_simt", "write_kv",
            "validate_block_tables", "merge_states", "paged_attention_v3_fp8",
            "write_kv_scaled", "append_kv", "write_kv_batch", "decode_layer_step",
-           "qk_norm_rope_append", "rope_table", "copy_blocks", "remap_block_tables", "shim_path"]
+           "paged_attention_shared", "qk_norm_rope_append", "rope_table", "copy_blocks",
+           "remap_block_tables", "shim_path"]
 
 
 def shim_path() -> Path:

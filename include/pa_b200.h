@@ -90,6 +90,9 @@ typedef enum pa_status {
 #define PA_DEVERR_RANGE 0x10     /* tensor-core prefill on an fp16 pool: a
                                     query element times scale is at or beyond
                                     the fp16 range (|x| >= 65520)             */
+#define PA_DEVERR_GROUP 0x20     /* shared-prefix decode: group_starts is not
+                                    0 <= s[0] <= s[1] <= ... <= num_seqs;
+                                    nothing was shared                         */
 
 PA_API int pa_abi_version(void);
 
@@ -510,6 +513,39 @@ PA_API int pa_qk_norm_rope_append(
     void* k_cache, void* v_cache, int kv_dtype, const float* k_scale, const float* v_scale,
     const int32_t* block_tables, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
     int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t max_blocks,
+    int32_t* dev_status, void* stream);
+
+/* Bytes of scratch pa_paged_attention_shared needs for these sizes. */
+PA_API int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_heads,
+                                    int64_t num_kv_heads, int64_t head_dim, int kv_dtype,
+                                    size_t* bytes);
+
+/* Decode of sequences that share a prefix, an addition (the reference's decode
+ * reads every sequence's whole context, kernels/paged_attn_v3.cu:192-261):
+ * the result of pa_paged_attention_v3, with the keys and values of a group's
+ * common prefix read once for all of its members.
+ *   Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1, and
+ * its members have the same first prefix_lens[g] tokens: for those positions
+ * their block-table rows lead to the same keys and values (the same pages, or
+ * copies of them, as a fork makes of its last page).  Any length, inside a page
+ * too.  What is used of it is at most the shortest member with tokens; the
+ * first such member's table row serves the group.  A sequence in no group is
+ * attended on its own.
+ *   group_starts: device int32 [num_groups + 1], 0 <= s[0] <= ... <= num_seqs
+ * (otherwise nothing is shared and PA_DEVERR_GROUP is reported); prefix_lens:
+ * device int32 [num_groups]; both may be NULL if num_groups is 0.
+ *   q, out [num_seqs, num_heads, head_dim] of io_dtype, which is kv_dtype:
+ * PA_DTYPE_F16 or PA_DTYPE_BF16; fp32 sums; the softmax weights are rounded to
+ * that type for their product with V, out once at the end.  lse (nullable)
+ * fp32 [num_seqs, num_heads].  A sequence with context_lens[b] <= 0 yields NaN
+ * and lse -inf.  head_dim in {32, 64, 128, 256}; any block_size >= 1;
+ * num_blocks * block_size * num_kv_heads < 2^32. */
+PA_API int pa_paged_attention_shared(
+    void* out, float* lse, const void* q, int io_dtype, const void* k_cache, const void* v_cache,
+    int kv_dtype, const int32_t* block_tables, const int32_t* context_lens,
+    const int32_t* group_starts, const int32_t* prefix_lens, int64_t num_seqs, int64_t num_groups,
+    int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+    int64_t num_blocks, int64_t max_blocks, double scale, void* workspace, size_t workspace_bytes,
     int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus

@@ -50,3 +50,28 @@ def _append(io=2, kv=2, T=1, seqs=1, rot=64, D=64, q=P, pos=P, cs=P, seq=P, wdt=
 ])
 def test_qk_norm_rope_append(kw, want):
     assert _append(**kw) == want
+
+
+def _shared(q=P, kv=1, io=1, B=3, NG=1, H=8, HKV=2, D=64, BS=16, gs=P, pl=P, ctx=P):
+    return _lib.call("pa_paged_attention_shared", P, None, q, io, P, P, kv, P, ctx, gs, pl, B, NG, H, HKV, D, BS, 8, 4,
+                     0.125, None, 0, None, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    ({"B": -1}, BAD), ({"NG": -1}, BAD), ({"H": 0}, BAD), ({"H": 9}, _lib.PA_ERR_NUM_HEADS),
+    ({"D": 96}, _lib.PA_ERR_HEAD_DIM), ({"kv": 0, "io": 0}, _lib.PA_ERR_DTYPE), ({"kv": 4}, _lib.PA_ERR_DTYPE),
+    ({"io": 2}, _lib.PA_ERR_DTYPE), ({"BS": 0}, BAD), ({"q": None}, BAD), ({"ctx": None}, BAD), ({"gs": None}, BAD),
+    ({"pl": None}, BAD), ({"q": ctypes.c_void_p(18)}, _lib.PA_ERR_ALIGNMENT), ({"BS": 1 << 31}, _lib.PA_ERR_TOO_LARGE),
+    ({"B": 1 << 32}, _lib.PA_ERR_TOO_LARGE), ({"B": 0, "q": None}, _lib.PA_OK),
+])
+def test_paged_attention_shared(kw, want):
+    assert _shared(**kw) == want
+
+
+def test_shared_workspace_size():
+    n = ctypes.c_size_t(7)
+    size = lambda *a: _lib.call("pa_shared_workspace_size", *a, ctypes.byref(n))  # noqa: E731
+    assert size(0, 0, 8, 2, 64, 1) == _lib.PA_OK and n.value == 0
+    assert size(3, 1, 9, 2, 64, 1) == _lib.PA_ERR_NUM_HEADS
+    assert size(3, 1, 8, 2, 64, 3) == _lib.PA_ERR_DTYPE
+    assert _lib.call("pa_shared_workspace_size", 3, 1, 8, 2, 64, 1, None) == BAD
