@@ -10,9 +10,9 @@
 // instead of once a sequence.
 //
 // Three launches, chained with programmatic dependent launch: a plan (one
-// CTA: the groups' usable prefixes, and the work cut into items of nearly
-// equal length), the attention itself (one warp per item), and the merge of
-// the items' partials.
+// CTA: the groups' usable prefixes and running counts of the work), the
+// attention itself (every warp takes an equal run of the work), and the merge
+// of the partials.
 #include <algorithm>
 #include <mutex>
 #include <vector>
@@ -25,22 +25,25 @@ namespace shared {
 constexpr int KT = 16;    // keys per tile
 constexpr int ROWS = 16;  // query rows per item (the M of one mma)
 
-// What a warp computes: rows r0 .. r0 + nrows - 1 of a unit (row r: sequence
-// b0 + r / G, head kvh * G + r % G) against keys t0 .. t1 - 1 of table row
-// `table`; partials go to rows prow .. prow + nrows - 1.
-struct Item {
-  int32_t table, b0, r0, nrows, kvh, t0, t1, prow;
+// The work, counted in tiles of KT keys: first the groups' prefixes, then the
+// sequences' own tokens.  A unit is one (group or sequence, KV head, tile of
+// rows); its tiles are consecutive, and the units of a group or sequence too,
+// in the order (KV head, tile of rows).  The `warps` workers of a launch take
+// equal consecutive runs of the total, worker w the tiles
+// [w T / W, (w + 1) T / W), so a unit is cut where a worker's run ends.  A piece
+// is the overlap of unit u and worker w; u + w grows strictly from piece to
+// piece, so it numbers the pieces' slots for partials, with no table of them.
+struct Group {
+  int64_t tile0;                // first tile
+  int32_t b0, n, table, prefix; // members b0 .. b0 + n - 1; table row that serves; tokens shared
+  int32_t unit0, pad;           // first unit
 };
-
-// Where a sequence's partials are: piece c of its prefix for KV head kv at row
-// pre_row + (kv * n_pre + c) * pre_rows + g, of its own tokens at
-// own_row + (kv * n_own + c) * G + g.
-struct SeqPlan {
-  int32_t n_pre, pre_row, pre_rows, n_own, own_row, ctx, pad[2];
+struct Seq {
+  int64_t tile0;
+  int32_t from, ctx, group, pad;  // own tokens from .. ctx - 1; its group or -1
 };
-
-struct GroupPlan {
-  int32_t b0, n, table, prefix;
+struct Totals {
+  int64_t prefix_tiles, tiles, workers;
 };
 
 struct Params {
@@ -54,175 +57,162 @@ struct Params {
   int32_t warps;    // warps of the attention launch
   int32_t bs_shift; // log2(BS) if BS is a power of two, else -1
   // workspace
-  int32_t* n_items;
-  GroupPlan* groups;
-  SeqPlan* seqs;
-  Item* items;
+  Totals* totals;
+  Group* groups;
+  Seq* seqs;
   float2* part_ml;  // (running max in log2 units, sum)
   float* part_o;
+  int64_t own_row0; // first partial row of the sequences' own units
   int32_t* dev_status;
 };
 
-__device__ __forceinline__ int32_t cdiv(int32_t a, int32_t b) { return (a + b - 1) / b; }
+__host__ __device__ __forceinline__ int32_t cdiv(int32_t a, int32_t b) { return (a + b - 1) / b; }
+
+// Worker w's first tile, and the worker of tile x, for T tiles over W workers.
+__device__ __forceinline__ int64_t first_tile(int64_t w, int64_t T, int64_t W) { return w * T / W; }
+__device__ __forceinline__ int64_t worker_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W - 1) / T; }
 
 // ---------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------
 
 constexpr int kPlanThreads = 1024;
+constexpr int kMinTiles = 2;  // tiles per worker when there are few
 
-// Exclusive scan of (a, b) over the block, with running totals in `base`.
-__device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sums, int2& base) {
+// Exclusive scan of (a, b) over the block on top of the running totals `base`.
+struct Pair {
+  int64_t a, b;
+};
+__device__ __forceinline__ Pair block_scan(Pair x, Pair* warp_sums, Pair& base) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int2 s = x;
+  auto warp_scan = [&](Pair s) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
-    if (lane >= o) s.x += a, s.y += b;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o);
+      if (lane >= o) s.a += a, s.b += b;
+    }
+    return s;
+  };
+  const Pair s = warp_scan(x);
   __syncthreads();
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  if (warp == 0) {
-    int2 w = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, w.x, o), b = __shfl_up_sync(0xffffffffu, w.y, o);
-      if (lane >= o) w.x += a, w.y += b;
-    }
-    warp_sums[lane] = w;
-  }
+  if (warp == 0) warp_sums[lane] = warp_scan(warp_sums[lane]);
   __syncthreads();
-  const int2 before = warp ? warp_sums[warp - 1] : make_int2(0, 0);
-  const int2 r = make_int2(base.x + before.x + s.x - x.x, base.y + before.y + s.y - x.y);
-  base.x += warp_sums[31].x;
-  base.y += warp_sums[31].y;
+  const Pair before = warp ? warp_sums[warp - 1] : Pair{0, 0};
+  const Pair r = {base.a + before.a + s.a - x.a, base.b + before.b + s.b - x.b};
+  base.a += warp_sums[31].a;
+  base.b += warp_sums[31].b;
   return r;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ Params p) {
-  __shared__ int2 sums[32];
-  __shared__ int32_t bad_groups;
-  __shared__ unsigned long long total_tiles;
+  __shared__ Pair sums[32];
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
   const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
-  const int32_t own_tiles_y = cdiv(G, ROWS);
-  if (tid == 0) bad_groups = 0, total_tiles = 0;
-  __syncthreads();
-  // group bounds that are not 0 <= s_0 <= s_1 <= ... <= B: no sharing at all
-  for (int32_t g = tid; g < NG; g += kPlanThreads) {
-    const int32_t a = p.group_starts[g], b = p.group_starts[g + 1];
-    if (a < 0 || b < a || b > B) bad_groups = 1;
-  }
-  __syncthreads();
-  if (bad_groups && tid == 0) report(p.dev_status, PA_DEVERR_GROUP);
+  const int32_t own_y = cdiv(G, ROWS);
   auto context = [&](int32_t b) {
     const int32_t c = p.context_lens[b];
     if (c > max_ctx) report(p.dev_status, PA_DEVERR_CONTEXT);
     return min(max(c, 0), max_ctx);
   };
+  // group bounds that are not 0 <= s_0 <= s_1 <= ... <= B: no sharing at all
+  int bad = 0;
+  for (int32_t g = tid; g < NG; g += kPlanThreads) {
+    const int32_t a = p.group_starts[g], b = p.group_starts[g + 1];
+    bad |= a < 0 || b < a || b > B;
+  }
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0) report(p.dev_status, PA_DEVERR_GROUP);
+  const int32_t groups = bad ? 0 : NG;
+  for (int32_t b = tid; b < B; b += kPlanThreads) p.seqs[b].group = -1;
+  __syncthreads();
   // a group's usable prefix: no longer than any member that has tokens; the
   // first such member's table row serves it.  One member alone shares nothing.
-  const int32_t groups = bad_groups ? 0 : NG;
-  unsigned long long tiles = 0;
   for (int32_t g = warp; g < groups; g += kPlanThreads / 32) {
     const int32_t a = p.group_starts[g], e = p.group_starts[g + 1];
     int32_t least = 0x7fffffff, first = 0x7fffffff, live = 0;
     for (int32_t b = a + lane; b < e; b += 32) {
       const int32_t c = context(b);
       if (c > 0) least = min(least, c), first = min(first, b), ++live;
+      p.seqs[b].group = g;
     }
     least = __reduce_min_sync(0xffffffffu, least);
     first = __reduce_min_sync(0xffffffffu, first);
     live = __reduce_add_sync(0xffffffffu, live);
-    const int32_t prefix = live > 1 ? max(0, min(p.prefix_lens[g], least)) : 0;
     if (lane == 0) {
-      p.groups[g] = GroupPlan{a, e - a, first, prefix};
-      tiles += (unsigned long long)HKV * cdiv((e - a) * G, ROWS) * cdiv(prefix, KT);
+      Group& gp = p.groups[g];
+      gp.b0 = a;
+      gp.n = e - a;
+      gp.table = first;
+      gp.prefix = live > 1 ? max(0, min(p.prefix_lens[g], least)) : 0;
     }
   }
   __syncthreads();
-  // the group of sequence b (largest g with group_starts[g] <= b), -1: none
-  auto group_of = [&](int32_t b) -> int32_t {
-    if (groups == 0 || b < p.group_starts[0] || b >= p.group_starts[groups]) return -1;
-    int32_t lo = 0, hi = groups;
-    while (hi - lo > 1) {
-      const int32_t m = (lo + hi) >> 1;
-      if (p.group_starts[m] <= b) lo = m;
-      else hi = m;
-    }
-    return lo;
-  };
-  for (int32_t b = tid; b < B; b += kPlanThreads) {
-    const int32_t g = group_of(b), ctx = context(b);
-    const int32_t from = g >= 0 ? min(p.groups[g].prefix, ctx) : 0;
-    tiles += (unsigned long long)HKV * own_tiles_y * cdiv(ctx - from, KT);
-  }
-  atomicAdd(&total_tiles, tiles);
-  __syncthreads();
-  // tiles per item: the whole work over the warps of the launch
-  const int32_t C = (int32_t)max((total_tiles + p.warps - 1) / p.warps, 1ull);
-
-  int2 base = make_int2(0, 0);  // (items, partial rows) so far
+  Pair base = {0, 0};  // tiles and units so far
   for (int32_t g0 = 0; g0 < groups; g0 += kPlanThreads) {
     const int32_t g = g0 + tid;
-    GroupPlan gp = {0, 0, 0, 0};
-    if (g < groups) gp = p.groups[g];
-    const int32_t nt = cdiv(gp.prefix, KT), n = cdiv(nt, C), rows = gp.n * G, ry = cdiv(rows, ROWS);
-    const int2 at = block_scan(make_int2(n * HKV * ry, n * HKV * rows), sums, base);
-    if (n > 0) {
-      int32_t i = at.x;
-      for (int32_t kv = 0; kv < HKV; ++kv)
-        for (int32_t c = 0; c < n; ++c)
-          for (int32_t y = 0; y < ry; ++y)
-            p.items[i++] = Item{gp.table, gp.b0, y * ROWS, min(ROWS, rows - y * ROWS), kv,
-                                (int32_t)((int64_t)nt * c / n) * KT,
-                                min(gp.prefix, (int32_t)((int64_t)nt * (c + 1) / n) * KT),
-                                at.y + (kv * n + c) * rows + y * ROWS};
+    Pair x = {0, 0};
+    if (g < groups) {
+      x.b = (int64_t)HKV * cdiv(p.groups[g].n * G, ROWS);
+      x.a = x.b * cdiv(p.groups[g].prefix, KT);
     }
-    if (g < groups)
-      for (int32_t m = 0; m < gp.n; ++m) {
-        SeqPlan& sp = p.seqs[gp.b0 + m];
-        sp.n_pre = n;
-        sp.pre_row = at.y + m * G;
-        sp.pre_rows = rows;
-      }
+    const Pair at = block_scan(x, sums, base);
+    if (g < groups) {
+      p.groups[g].tile0 = at.a;
+      p.groups[g].unit0 = (int32_t)at.b;
+    }
   }
-  __syncthreads();
+  const int64_t prefix_tiles = base.a;
   for (int32_t b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int32_t b = b0 + tid;
-    int32_t g = -1, ctx = 0, from = 0;
+    Pair x = {0, 0};
+    int32_t ctx = 0, from = 0;
     if (b < B) {
-      g = group_of(b);
+      const int32_t g = p.seqs[b].group;
       ctx = context(b);
-      from = g >= 0 ? min(p.groups[g].prefix, ctx) : 0;
+      if (g >= 0) from = min(p.groups[g].prefix, ctx);
+      x.a = (int64_t)HKV * own_y * cdiv(ctx - from, KT);
     }
-    const int32_t nt = cdiv(ctx - from, KT), n = cdiv(nt, C);
-    const int2 at = block_scan(make_int2(n * HKV * own_tiles_y, n * HKV * G), sums, base);
+    const Pair at = block_scan(x, sums, base);
     if (b < B) {
-      SeqPlan& sp = p.seqs[b];
-      if (g < 0 || ctx == 0) sp.n_pre = 0;
-      sp.n_own = n;
-      sp.own_row = at.y;
-      sp.ctx = ctx;
-      int32_t i = at.x;
-      for (int32_t kv = 0; kv < HKV; ++kv)
-        for (int32_t c = 0; c < n; ++c)
-          for (int32_t y = 0; y < own_tiles_y; ++y)
-            p.items[i++] = Item{b, b, y * ROWS, min(ROWS, G - y * ROWS), kv,
-                                from + (int32_t)((int64_t)nt * c / n) * KT,
-                                min(ctx, from + (int32_t)((int64_t)nt * (c + 1) / n) * KT),
-                                at.y + (kv * n + c) * G + y * ROWS};
+      p.seqs[b].tile0 = at.a;
+      p.seqs[b].from = from;
+      p.seqs[b].ctx = ctx;
     }
   }
-  if (tid == 0) *p.n_items = base.x;
+  if (tid == 0)
+    *p.totals = Totals{prefix_tiles, base.a,
+                       min((int64_t)p.warps, max((base.a + kMinTiles - 1) / kMinTiles, (int64_t)1))};
 }
 
 // ---------------------------------------------------------------------------
-// attention: one warp per item
+// attention: one warp per worker
 // ---------------------------------------------------------------------------
+
+// What a warp computes at a time: rows r0 .. r0 + nrows - 1 of a unit (row r:
+// sequence b0 + r / G, head kvh * G + r % G) against keys t0 .. t1 - 1 of table
+// row `table`; partials from row prow on.
+struct Item {
+  int32_t table, b0, r0, nrows, kvh, t0, t1, prow;
+};
+
+// The last of n entries (their tile0 rising from at most x) with tile0 <= x.
+// All lanes probe at once: two steps for 1024 entries.
+template <typename E>
+__device__ __forceinline__ int32_t find(const E* e, int32_t n, int64_t x, int lane) {
+  int32_t lo = 0, len = n;  // the answer is in [lo, lo + len)
+  while (len > 1) {
+    const int32_t step = (len + 31) / 32, at = lo + lane * step;
+    const uint32_t m = __ballot_sync(0xffffffffu, lane * step < len && e[at].tile0 <= x);
+    const int32_t k = 31 - __clz(m);
+    len = min(step, len - k * step);
+    lo += k * step;
+  }
+  return lo;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -288,19 +278,59 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const 
   pdl_wait();
   pdl_trigger();
   const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-  const int32_t n_items = *p.n_items;
+  const Totals tot = *p.totals;
   // rows of a tile sit `D * 2` bytes apart with their 16-byte chunks permuted
   // by the row, so the eight rows of a matrix load fall on different banks
   auto chunk_at = [](int row, int c) -> uint32_t {
     return (uint32_t)(row * (D * 2) + ((c ^ (CH >= 8 ? (row & 7) : ((row >> 1) & 3))) << 4));
   };
-  // consecutive items go to different SMs
-  for (int32_t it = warp * gridDim.x + blockIdx.x; it < n_items; it += p.warps) {
-    const int4 w0 = reinterpret_cast<const int4*>(p.items + it)[0];
-    const int4 w1 = reinterpret_cast<const int4*>(p.items + it)[1];
-    const Item im = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    const int n_tiles = (im.t1 - im.t0 + KT - 1) / KT;
+  // consecutive workers sit on different SMs
+  const int64_t worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= tot.workers) return;
+  const int32_t HKV = (int32_t)p.HKV, own_y = cdiv(p.G, ROWS);
+  int64_t x = first_tile(worker, tot.tiles, tot.workers);
+  const int64_t end = first_tile(worker + 1, tot.tiles, tot.workers);
+  int32_t at = -1;  // the group or sequence of tile x; of which is `x < prefix_tiles`
+  bool in_prefix = x < tot.prefix_tiles;
+  if (x < end)
+    at = in_prefix ? find(p.groups, (int32_t)p.NG, x, lane) : find(p.seqs, (int32_t)p.B, x, lane);
+  while (x < end) {
+    if (in_prefix && x >= tot.prefix_tiles) in_prefix = false, at = 0;
+    Item im;
+    int64_t left;  // tiles of the unit from x on
+    if (in_prefix) {
+      const Group gp = p.groups[at];
+      const int32_t rows = gp.n * p.G, ry = cdiv(rows, ROWS), nt = cdiv(gp.prefix, KT);
+      const int64_t done = x - gp.tile0;
+      if (done >= (int64_t)HKV * ry * nt) { ++at; continue; }
+      const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
+      left = min((int64_t)(nt - j), end - x);
+      im.table = gp.table;
+      im.b0 = gp.b0;
+      im.kvh = u / ry;
+      im.r0 = (u - im.kvh * ry) * ROWS;
+      im.nrows = min(ROWS, rows - im.r0);
+      im.t0 = j * KT;
+      im.t1 = min(gp.prefix, im.t0 + (int32_t)left * KT);
+      im.prow = (int32_t)((gp.unit0 + u + worker) * ROWS);
+    } else {
+      const Seq sp = p.seqs[at];
+      const int32_t nt = cdiv(sp.ctx - sp.from, KT);
+      const int64_t done = x - sp.tile0;
+      if (done >= (int64_t)HKV * own_y * nt) { ++at; continue; }
+      const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
+      left = min((int64_t)(nt - j), end - x);
+      im.table = im.b0 = at;
+      im.kvh = u / own_y;
+      im.r0 = (u - im.kvh * own_y) * ROWS;
+      im.nrows = min(ROWS, p.G - im.r0);
+      im.t0 = sp.from + j * KT;
+      im.t1 = min(sp.ctx, im.t0 + (int32_t)left * KT);
+      im.prow = (int32_t)(p.own_row0 + ((int64_t)at * HKV * own_y + u + worker) * min(p.G, ROWS));
+    }
+    x += left;
     const int32_t* table = p.block_tables + (int64_t)im.table * p.MB;
+    const int n_tiles = (im.t1 - im.t0 + KT - 1) / KT;
 
     // pool row (in rows of D elements) of token t0 + 16 j + lane, lanes 0-15
     auto row_of = [&](int j) -> uint32_t {
@@ -458,11 +488,31 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   if (row >= p.B * p.H) return;
   const int64_t b = row / p.H;
   const int32_t h = (int32_t)(row % p.H), kv = h / p.G, g = h % p.G;
-  const SeqPlan sp = p.seqs[b];
-  const int n = sp.n_pre + sp.n_own;
+  const int32_t own_y = cdiv(p.G, ROWS), own_rows = min(p.G, ROWS);
+  const Totals tot = *p.totals;
+  const Seq sp = p.seqs[b];
+  // this row's pieces: slot0 + c * step, first of its prefix unit, then of its own
+  int64_t pre0 = 0, own0 = 0;
+  int32_t n_pre = 0, n_own = 0;
+  if (sp.group >= 0 && sp.from > 0) {
+    const Group gp = p.groups[sp.group];
+    const int32_t rows = gp.n * p.G, ry = cdiv(rows, ROWS), nt = cdiv(gp.prefix, KT);
+    const int32_t r = ((int32_t)b - gp.b0) * p.G + g, u = kv * ry + r / ROWS;
+    const int64_t a = gp.tile0 + (int64_t)u * nt;
+    const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
+    n_pre = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
+    pre0 = (gp.unit0 + u + w0) * ROWS + r % ROWS;
+  }
+  if (sp.ctx > sp.from) {
+    const int32_t nt = cdiv(sp.ctx - sp.from, KT), u = kv * own_y + g / ROWS;
+    const int64_t a = sp.tile0 + (int64_t)u * nt;
+    const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
+    n_own = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
+    own0 = p.own_row0 + (b * p.HKV * own_y + u + w0) * own_rows + g % ROWS;
+  }
+  const int n = n_pre + n_own;
   auto piece = [&](int c) -> int64_t {
-    return c < sp.n_pre ? (int64_t)sp.pre_row + (int64_t)(kv * sp.n_pre + c) * sp.pre_rows + g
-                        : (int64_t)sp.own_row + (int64_t)(kv * sp.n_own + c - sp.n_pre) * p.G + g;
+    return c < n_pre ? pre0 + (int64_t)c * ROWS : own0 + (int64_t)(c - n_pre) * own_rows;
   };
   float M = -INFINITY;
   for (int c = lane; c < n; c += 32) M = fmaxf(M, p.part_ml[piece(c)].x);
@@ -491,26 +541,26 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 // ---------------------------------------------------------------------------
 
 struct Layout {
-  size_t groups, seqs, items, ml, o, total;
+  int64_t own_row0;
+  size_t groups, seqs, ml, o, total;
 };
 
 static int warps_per_cta(int64_t D) {
   return D == 32 ? Cfg<32>::WARPS : D == 64 ? Cfg<64>::WARPS : D == 128 ? Cfg<128>::WARPS : Cfg<256>::WARPS;
 }
 
-// Items: a unit (rows x KV head) of x tiles makes ceil(x / C) of them with
-// C >= sum x / warps, so at most warps + units in all; an item has at most
-// ROWS rows, so the partial rows are at most ROWS x warps + the units' rows.
+// Slots for partials: unit + worker < units + workers, for prefixes with ROWS
+// rows each, for sequences' own units with min(G, ROWS).
 static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, Layout* y) {
   const int64_t G = H / HKV, warps = (int64_t)sms * warps_per_cta(D);
-  const int64_t units = HKV * ((B * G + ROWS - 1) / ROWS + NG + B * ((G + ROWS - 1) / ROWS));
-  const int64_t items = warps + units, rows = ROWS * warps + 2 * B * H;
-  if (items >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
+  const int64_t pre_units = NG ? HKV * (B * G / ROWS + NG) : 0, own_units = B * HKV * ((G + ROWS - 1) / ROWS);
+  y->own_row0 = NG ? (pre_units + warps) * ROWS : 0;
+  const int64_t rows = y->own_row0 + (own_units + warps) * std::min<int64_t>(G, ROWS);
+  if (rows >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   y->groups = 256;
-  y->seqs = y->groups + up((size_t)NG * sizeof(GroupPlan));
-  y->items = y->seqs + up((size_t)B * sizeof(SeqPlan));
-  y->ml = y->items + up((size_t)items * sizeof(Item));
+  y->seqs = y->groups + up((size_t)NG * sizeof(Group));
+  y->ml = y->seqs + up((size_t)B * sizeof(Seq));
   y->o = y->ml + up((size_t)rows * sizeof(float2));
   y->total = y->o + up((size_t)rows * D * sizeof(float));
   return PA_OK;
@@ -649,10 +699,10 @@ extern "C" int pa_paged_attention_shared(
   p.bs_shift = -1;
   if ((block_size & (block_size - 1)) == 0)
     for (p.bs_shift = 0; (int64_t(1) << p.bs_shift) < block_size; ++p.bs_shift) {}
-  p.n_items = reinterpret_cast<int32_t*>(ws);
-  p.groups = reinterpret_cast<shared::GroupPlan*>(ws + y.groups);
-  p.seqs = reinterpret_cast<shared::SeqPlan*>(ws + y.seqs);
-  p.items = reinterpret_cast<shared::Item*>(ws + y.items);
+  p.totals = reinterpret_cast<shared::Totals*>(ws);
+  p.groups = reinterpret_cast<shared::Group*>(ws + y.groups);
+  p.seqs = reinterpret_cast<shared::Seq*>(ws + y.seqs);
+  p.own_row0 = y.own_row0;
   p.part_ml = reinterpret_cast<float2*>(ws + y.ml);
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.dev_status = dev_status;
