@@ -27,6 +27,8 @@ struct Params {
   int64_t T, H, HKV, MB, n_seqs, BS, NB;
   char *q_out, *k_cache, *v_cache;
   const float *k_scale, *v_scale;  // FP8 pools: [HKV], null = 1
+  int32_t lph_shift;  // log2(head_dim / 8)
+  int32_t bs_shift;   // log2(BS) if BS is a power of two, else -1
   int32_t* dev_status;
 };
 
@@ -43,125 +45,314 @@ template <> __device__ __forceinline__ __nv_fp8_e4m3 from_f32<__nv_fp8_e4m3>(flo
   return r;
 }
 
-// One warp per (token, head) of the H + 2 HKV heads; lane holds elements
-// lane + 32 i.
-template <typename S, typename P, int D>
-__global__ void __launch_bounds__(256) qk_append_kernel(const __grid_constant__ Params p) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31;
+// Where token t's K and V rows go: the pool row, or -1 for none (padding, or a
+// place outside the table or pool, which is reported if `tell`).
+__device__ __forceinline__ int64_t pool_row(const Params& p, int64_t t, int64_t pos, bool tell) {
+  if (pos < 0) return -1;
+  if (pos >= p.max_pos) {
+    if (tell) report(p.dev_status, PA_DEVERR_CONTEXT);
+    return -1;
+  }
+  const int64_t seq = p.seq_ids ? p.seq_ids[t] : t;
+  const int64_t page = p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.BS;
+  if (seq < 0 || seq >= p.n_seqs || page >= p.MB) {
+    if (tell) report(p.dev_status, PA_DEVERR_CONTEXT);
+    return -1;
+  }
+  const int64_t blk = p.tables[seq * p.MB + page];
+  if (blk < 0 || blk >= p.NB) {
+    if (tell) report(p.dev_status, PA_DEVERR_BLOCK_ID);
+    return -1;
+  }
+  return blk * p.BS + (pos - page * p.BS);
+}
+
+// One element of a turned pair: x cos + other sin (sin negated for the first
+// of the pair).  Pinned, as is the order of the sums of squares (a lane's four
+// pairs of elements, then a tree over the lanes), so that every variant gives
+// the same bits.
+__device__ __forceinline__ float turned(float x, float other, float c, float s) {
+  return fmaf(other, s, __fmul_rn(x, c));
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 pa, pb, pd;\n\tmov.b64 pa, {%2, %3};\n\tmov.b64 pb, {%4, %5};\n\t"
+      "mul.rn.f32x2 pd, pa, pb;\n\tmov.b64 {%0, %1}, pd;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// A lane's eight elements of a head are two runs of four, from a and from b on:
+// for pairs (i, i + R / 2) the two halves' same places, so that a pair never
+// leaves its lane; otherwise neighbouring runs.
+struct Place {
+  int a, b;
+  bool turns;
+};
+__device__ __forceinline__ Place place(const Params& p, int sub) {
+  const bool turns = sub * 8 < p.R;
+  if (turns && !p.interleaved) return {4 * sub, p.R / 2 + 4 * sub, true};
+  return {8 * sub, 8 * sub + 4, turns};
+}
+
+// Four elements of a source row as loaded, and stores of four elements.
+template <typename S> struct Raw4;
+template <> struct Raw4<float> { using T = uint4; };
+template <> struct Raw4<__half> { using T = uint2; };
+template <> struct Raw4<__nv_bfloat16> { using T = uint2; };
+
+template <typename S> __device__ __forceinline__ void unpack4(const typename Raw4<S>::T& u, float2* f) {
+  if constexpr (sizeof(S) == 4) {
+    f[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else if constexpr (DTypeId<S>::value == PA_DTYPE_BF16) {  // the high half of an fp32
+    f[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
+    f[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+  } else {
+    f[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    f[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  }
+}
+template <typename P> __device__ __forceinline__ void store4(P* dst, const float2* f) {
+  if constexpr (DTypeId<P>::value == PA_DTYPE_BF16) {
+    __nv_bfloat162 v[2] = {__float22bfloat162_rn(f[0]), __float22bfloat162_rn(f[1])};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+  } else if constexpr (DTypeId<P>::value == PA_DTYPE_F16) {
+    __half2 v[2] = {__float22half2_rn(f[0]), __float22half2_rn(f[1])};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+  } else {
+    struct alignas(sizeof(P) >= 4 ? 16 : 4 * sizeof(P)) Four {
+      P x[4];
+    };
+    const Four v = {{from_f32<P>(f[0].x), from_f32<P>(f[0].y), from_f32<P>(f[1].x), from_f32<P>(f[1].y)}};
+    *reinterpret_cast<Four*>(dst) = v;
+  }
+}
+
+constexpr int kThreads = 128;
+constexpr int kBatch = 4;  // heads in flight per thread
+
+// One CTA per token.  D / 8 lanes hold a head, eight elements each, so the CTA
+// works on 1024 / D heads at a time and has four times as many in flight.  A
+// thread keeps its place in the head: the cosines and sines of its four pairs
+// and its eight weights are loaded once for all of its heads.  HBM-bound: a
+// token's q, k and v are read once and written once.
+template <typename S, typename P>
+__global__ void __launch_bounds__(kThreads) qk_append_kernel(const __grid_constant__ Params p) {
+  using R4 = typename Raw4<S>::T;
+  const int lph = 1 << p.lph_shift;  // lanes per head, D / 8
+  const int sub = threadIdx.x & (lph - 1), grp = threadIdx.x >> p.lph_shift;
+  const int groups = kThreads >> p.lph_shift;
+  const int warp_grp = (threadIdx.x & ~31) >> p.lph_shift;  // the warp's first group
+  const int D = lph * 8, H = (int)p.H, HKV = (int)p.HKV;
+  const int64_t t = blockIdx.x;
+  const Place at = place(p, sub);
+  const int64_t pos = p.positions[t];
+  S* const q_out = reinterpret_cast<S*>(p.q_out) + t * H * D;
+
+  if (pos < 0 || pos >= p.max_pos) {  // a padding token's q is zero, one past the table's is NaN
+    if (pos >= 0 && threadIdx.x == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
+    const float x = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+    const float2 y[2] = {make_float2(x, x), make_float2(x, x)};
+    for (int e = threadIdx.x * 4; e < H * D; e += kThreads * 4) store4<S>(q_out + e, y);
+    return;
+  }
+  const int64_t row = pool_row(p, t, pos, threadIdx.x == 0);
+
+  float2 c[2] = {}, s[2] = {};
+  if (at.turns) {
+    const float* cs = p.cos_sin + pos * p.R + 4 * sub;
+    const float4 x = *reinterpret_cast<const float4*>(cs), y = *reinterpret_cast<const float4*>(cs + p.R / 2);
+    c[0] = make_float2(x.x, x.y), c[1] = make_float2(x.z, x.w);
+    s[0] = make_float2(y.x, y.y), s[1] = make_float2(y.z, y.w);
+  }
+
+  // Every head of x[n heads]: norm, turn, `put`.
+  auto each = [&](const char* base, int64_t head_stride, int n, const char* w, bool turn, auto put) {
+    const S* src = reinterpret_cast<const S*>(base);
+    float2 g[4];
+    if (w) {
+      if (p.w_f32) {
+        unpack4<float>(*reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(w) + at.a), g);
+        unpack4<float>(*reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(w) + at.b), g + 2);
+      } else {
+        unpack4<S>(*reinterpret_cast<const R4*>(reinterpret_cast<const S*>(w) + at.a), g);
+        unpack4<S>(*reinterpret_cast<const R4*>(reinterpret_cast<const S*>(w) + at.b), g + 2);
+      }
+    }
+    for (int h0 = 0; h0 + warp_grp < n; h0 += kBatch * groups) {
+      R4 raw[kBatch][2];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = h0 + i * groups + grp;
+        raw[i][0] = raw[i][1] = R4{};
+        if (h < n) {
+          raw[i][0] = __ldcs(reinterpret_cast<const R4*>(src + h * head_stride + at.a));
+          raw[i][1] = __ldcs(reinterpret_cast<const R4*>(src + h * head_stride + at.b));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = h0 + i * groups + grp;
+        if (h0 + i * groups + warp_grp >= n) break;  // the whole warp leaves
+        float2 y[4];
+        unpack4<S>(raw[i][0], y);
+        unpack4<S>(raw[i][1], y + 2);
+        if (w) {
+          float2 q2 = mul2(y[0], y[0]);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) q2 = fma2(y[e], y[e], q2);
+          float sum = q2.x + q2.y;
+          for (int o = lph >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float r = rsqrtf(sum * (1.f / D) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = mul2(mul2(y[e], make_float2(r, r)), g[e]);
+        }
+        if (turn && at.turns) {
+          if (p.interleaved) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float cc = e & 1 ? c[e >> 1].y : c[e >> 1].x, ss = e & 1 ? s[e >> 1].y : s[e >> 1].x;
+              y[e] = make_float2(turned(y[e].x, y[e].y, cc, -ss), turned(y[e].y, y[e].x, cc, ss));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 a = y[e], b = y[e + 2];
+              y[e] = fma2(b, make_float2(-s[e].x, -s[e].y), mul2(a, c[e]));
+              y[e + 2] = fma2(a, s[e], mul2(b, c[e]));
+            }
+          }
+        }
+        if (h < n) put(h, y);
+      }
+    }
+  };
+  auto to_pool = [&](char* cache, const float* scale) {
+    P* dst = reinterpret_cast<P*>(cache) + row * HKV * D;
+    return [=](int h, float2 (&y)[4]) {
+      if constexpr (sizeof(P) == 1) {
+        const float qs = scale ? scale[h] : 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = make_float2(__fdiv_rn(y[e].x, qs), __fdiv_rn(y[e].y, qs));
+      }
+      store4<P>(dst + h * D + at.a, y);
+      store4<P>(dst + h * D + at.b, y + 2);
+    };
+  };
+  if (row >= 0) {
+    each(p.v + t * p.v_tok * sizeof(S), p.v_head, HKV, nullptr, false, to_pool(p.v_cache, p.v_scale));
+    each(p.k + t * p.k_tok * sizeof(S), p.k_head, HKV, p.k_weight, true, to_pool(p.k_cache, p.k_scale));
+  }
+  each(p.q + t * p.q_tok * sizeof(S), p.q_head, H, p.q_weight, true, [&](int h, float2 (&y)[4]) {
+    store4<S>(q_out + h * D + at.a, y);
+    store4<S>(q_out + h * D + at.b, y + 2);
+  });
+}
+
+// Any alignment and strides, and rotated parts that are no multiple of eight:
+// one warp per (token, head), D / 8 lanes with eight elements each, one access
+// an element, a pair's other element by a second load.
+template <typename S, typename P>
+__global__ void __launch_bounds__(kThreads) qk_append_any_kernel(const __grid_constant__ Params p) {
+  const int lane = threadIdx.x & 31, lph = 1 << p.lph_shift, D = 8 * lph;
   const int64_t heads = p.H + 2 * p.HKV;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (unit >= p.T * heads) return;
   const int64_t t = unit / heads, hh = unit % heads;
   const int kind = hh < p.H ? 0 : (hh < p.H + p.HKV ? 1 : 2);  // q, k, v
   const int64_t h = kind == 0 ? hh : (kind == 1 ? hh - p.H : hh - p.H - p.HKV);
   const int64_t pos = p.positions[t];
-  const bool known = pos >= 0 && pos < p.max_pos;
-
-  // the row of the pool
-  char* row = nullptr;
-  if (kind != 0) {
-    if (pos < 0) return;
-    if (!known) {
-      if (lane == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
-      return;
-    }
-    const int64_t seq = p.seq_ids ? p.seq_ids[t] : t;
-    const int64_t page = pos / p.BS;
-    if (seq < 0 || seq >= p.n_seqs || page >= p.MB) {
-      if (lane == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
-      return;
-    }
-    const int64_t blk = p.tables[seq * p.MB + page];
-    if (blk < 0 || blk >= p.NB) {
-      if (lane == 0) report(p.dev_status, PA_DEVERR_BLOCK_ID);
-      return;
-    }
-    row = (kind == 1 ? p.k_cache : p.v_cache) +
-          ((blk * p.BS + (pos - page * p.BS)) * p.HKV + h) * D * (int64_t)sizeof(P);
-  } else if (!known) {
-    // a padding token's q is zero, one past the table's is NaN
+  const bool known = pos >= 0 && pos < p.max_pos, mine = lane < lph;
+  const int64_t row = kind ? pool_row(p, t, pos, lane == 0) : 0;
+  if (row < 0) return;
+  Place at = place(p, lane);
+  if (p.R % 8) at = {8 * lane, 8 * lane + 4, false};
+  auto element = [&](int i) { return i < 4 ? at.a + i : at.b + i - 4; };
+  S* q_out = reinterpret_cast<S*>(p.q_out) + (t * p.H + h) * D;
+  if (!known) {  // a padding token's q is zero, one past the table's is NaN
     if (pos >= 0 && lane == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
-    S* out = reinterpret_cast<S*>(p.q_out) + (t * p.H + h) * D;
-    for (int i = 0; i < N; ++i) out[lane + 32 * i] = from_f32<S>(pos < 0 ? 0.f : __int_as_float(0x7fc00000));
+    for (int i = 0; i < 8 && mine; ++i) q_out[element(i)] = from_f32<S>(pos < 0 ? 0.f : __int_as_float(0x7fc00000));
     return;
   }
-
   const S* src = kind == 0   ? reinterpret_cast<const S*>(p.q) + t * p.q_tok + h * p.q_head
                  : kind == 1 ? reinterpret_cast<const S*>(p.k) + t * p.k_tok + h * p.k_head
                              : reinterpret_cast<const S*>(p.v) + t * p.v_tok + h * p.v_head;
-  float y[N];
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < N; ++i) y[i] = to_f32<S>(src[lane + 32 * i]);
+  for (int i = 0; i < 8; ++i) y[i] = mine ? to_f32<S>(src[element(i)]) : 0.f;
   if (kind != 2) {
     const char* w = kind == 0 ? p.q_weight : p.k_weight;
     float r = 1.f;
     if (w) {
-      float sum = 0.f;
+      float even = __fmul_rn(y[0], y[0]), odd = __fmul_rn(y[1], y[1]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum = fmaf(y[i], y[i], sum);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int i = 2; i < 8; i += 2) even = fmaf(y[i], y[i], even), odd = fmaf(y[i + 1], y[i + 1], odd);
+      float sum = even + odd;
+      for (int o = lph >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       r = rsqrtf(sum * (1.f / D) + p.eps);
     }
-    auto weight = [&](int e) -> float {
-      if (!w) return 1.f;
-      return p.w_f32 ? reinterpret_cast<const float*>(w)[e] : to_f32<S>(reinterpret_cast<const S*>(w)[e]);
+    auto normed = [&](float x, int e) -> float {
+      if (!w) return x;
+      const float g = p.w_f32 ? reinterpret_cast<const float*>(w)[e] : to_f32<S>(reinterpret_cast<const S*>(w)[e]);
+      return __fmul_rn(__fmul_rn(x, r), g);
     };
     const int half = p.R / 2;
     const float* cs = p.cos_sin + pos * p.R;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = lane + 32 * i;
-      const float x = y[i] * r * weight(e);
+    for (int i = 0; i < 8; ++i) {
+      const int e = element(i);
+      if (!mine) break;
+      y[i] = normed(y[i], e);
       if (e < p.R) {
         // the pair's other element, and whether this is its first
         const bool first = p.interleaved ? (e & 1) == 0 : e < half;
         const int other = p.interleaved ? e ^ 1 : (first ? e + half : e - half);
         const int a = p.interleaved ? e >> 1 : (first ? e : e - half);
-        const float xo = to_f32<S>(src[other]) * r * weight(other);
-        const float c = cs[a], s = cs[half + a];
-        y[i] = first ? x * c - xo * s : x * c + xo * s;
-      } else {
-        y[i] = x;
+        const float s = cs[half + a];
+        y[i] = turned(y[i], normed(to_f32<S>(src[other]), other), cs[a], first ? -s : s);
       }
     }
   }
+  if (!mine) return;
   if (kind == 0) {
-    S* out = reinterpret_cast<S*>(p.q_out) + (t * p.H + h) * D;
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[lane + 32 * i] = from_f32<S>(y[i]);
+    for (int i = 0; i < 8; ++i) q_out[element(i)] = from_f32<S>(y[i]);
   } else {
-    P* out = reinterpret_cast<P*>(row);
+    P* out = reinterpret_cast<P*>(kind == 1 ? p.k_cache : p.v_cache) + (row * p.HKV + h) * D;
     const float* sc = kind == 1 ? p.k_scale : p.v_scale;
     const float qs = sizeof(P) == 1 && sc ? sc[h] : 1.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      out[lane + 32 * i] = from_f32<P>(sizeof(P) == 1 ? __fdiv_rn(y[i], qs) : y[i]);
+    for (int i = 0; i < 8; ++i) out[element(i)] = from_f32<P>(sizeof(P) == 1 ? __fdiv_rn(y[i], qs) : y[i]);
   }
 }
 
 template <typename S, typename P>
-static int launch_typed(const Params& p, int64_t D, cudaStream_t s) {
-  const int64_t ctas = (p.T * (p.H + 2 * p.HKV) + 7) / 8;
-  if (ctas > (int64_t(1) << 31) - 1) return PA_ERR_TOO_LARGE;
-  switch (D) {
-    case 32: qk_append_kernel<S, P, 32><<<(unsigned)ctas, 256, 0, s>>>(p); break;
-    case 64: qk_append_kernel<S, P, 64><<<(unsigned)ctas, 256, 0, s>>>(p); break;
-    case 128: qk_append_kernel<S, P, 128><<<(unsigned)ctas, 256, 0, s>>>(p); break;
-    default: qk_append_kernel<S, P, 256><<<(unsigned)ctas, 256, 0, s>>>(p); break;
+static int launch_typed(const Params& p, cudaStream_t s) {
+  const int64_t D = int64_t(8) << p.lph_shift, heads = p.H + 2 * p.HKV;
+  auto strides = [](int64_t tok, int64_t head) { return (tok * sizeof(S)) % 16 == 0 && (head * sizeof(S)) % 16 == 0; };
+  const bool wide = aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && strides(p.q_tok, p.q_head) &&
+                    strides(p.k_tok, p.k_head) && strides(p.v_tok, p.v_head) && aligned16(p.q_out) &&
+                    aligned16(p.k_cache) && aligned16(p.v_cache) && aligned16(p.q_weight) &&
+                    aligned16(p.k_weight) && aligned16(p.cos_sin) && p.R % 8 == 0;
+  if (wide && p.T <= 0x7fffffff && p.H * D <= 0x7fffffff) {
+    qk_append_kernel<S, P><<<(unsigned)p.T, kThreads, 0, s>>>(p);
+  } else {
+    const int64_t ctas = (p.T * heads + kThreads / 32 - 1) / (kThreads / 32);
+    if (ctas > 0x7fffffff) return PA_ERR_TOO_LARGE;
+    qk_append_any_kernel<S, P><<<(unsigned)ctas, kThreads, 0, s>>>(p);
   }
   return cuda_status(cudaGetLastError());
 }
 
 template <typename S>
-static int launch_src(const Params& p, int pool_dtype, int64_t D, cudaStream_t s) {
+static int launch_src(const Params& p, int pool_dtype, cudaStream_t s) {
   switch (pool_dtype) {
-    case PA_DTYPE_F16: return launch_typed<S, __half>(p, D, s);
-    case PA_DTYPE_BF16: return launch_typed<S, __nv_bfloat16>(p, D, s);
-    case PA_DTYPE_F32: return launch_typed<S, float>(p, D, s);
-    case PA_DTYPE_F64: return launch_typed<S, double>(p, D, s);
-    default: return launch_typed<S, __nv_fp8_e4m3>(p, D, s);
+    case PA_DTYPE_F16: return launch_typed<S, __half>(p, s);
+    case PA_DTYPE_BF16: return launch_typed<S, __nv_bfloat16>(p, s);
+    case PA_DTYPE_F32: return launch_typed<S, float>(p, s);
+    case PA_DTYPE_F64: return launch_typed<S, double>(p, s);
+    default: return launch_typed<S, __nv_fp8_e4m3>(p, s);
   }
 }
 
@@ -226,11 +417,15 @@ extern "C" int pa_qk_norm_rope_append(
   p.v_cache = static_cast<char*>(v_cache);
   p.k_scale = k_scale;
   p.v_scale = v_scale;
+  for (p.lph_shift = 2; (int64_t(8) << p.lph_shift) < head_dim; ++p.lph_shift) {}
+  p.bs_shift = -1;
+  if ((block_size & (block_size - 1)) == 0)
+    for (p.bs_shift = 0; (int64_t(1) << p.bs_shift) < block_size; ++p.bs_shift) {}
   p.dev_status = dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (io_dtype) {
-    case PA_DTYPE_F32: return qkappend::launch_src<float>(p, kv_dtype, head_dim, s);
-    case PA_DTYPE_F16: return qkappend::launch_src<__half>(p, kv_dtype, head_dim, s);
-    default: return qkappend::launch_src<__nv_bfloat16>(p, kv_dtype, head_dim, s);
+    case PA_DTYPE_F32: return qkappend::launch_src<float>(p, kv_dtype, s);
+    case PA_DTYPE_F16: return qkappend::launch_src<__half>(p, kv_dtype, s);
+    default: return qkappend::launch_src<__nv_bfloat16>(p, kv_dtype, s);
   }
 }
