@@ -129,7 +129,7 @@ template <typename P> __device__ __forceinline__ void store4(P* dst, const float
   }
 }
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 64;
 constexpr int kBatch = 4;  // heads in flight per thread
 
 // One CTA per token.  D / 8 lanes hold a head, eight elements each, so the CTA

@@ -9,75 +9,27 @@
 // rows of one product, and each K/V element of the prefix is read once a group
 // instead of once a sequence.
 //
-// Three launches, chained with programmatic dependent launch: a plan (one
-// CTA: the groups' usable prefixes and running counts of the work), the
-// attention itself (every warp takes an equal run of the work), and the merge
-// of the partials.
+// Launches, chained with programmatic dependent launch: a plan (one CTA: the
+// groups' usable prefixes and running counts of the work), the prefixes of
+// groups with many rows on the tensor cores (shared_tc.cu), all other prefixes
+// and the sequences' own tokens (every warp takes an equal run of the work),
+// and the merge of the partials.
 #include <algorithm>
 #include <mutex>
 #include <vector>
 
-#include "common.cuh"
+#include "shared.cuh"
 
 namespace pa {
 namespace shared {
-
-constexpr int KT = 16;    // keys per tile
-constexpr int ROWS = 16;  // query rows per item (the M of one mma)
-
-// The work, counted in tiles of KT keys: first the groups' prefixes, then the
-// sequences' own tokens.  A unit is one (group or sequence, KV head, tile of
-// rows); its tiles are consecutive, and the units of a group or sequence too,
-// in the order (KV head, tile of rows).  The `warps` workers of a launch take
-// equal consecutive runs of the total, worker w the tiles
-// [w T / W, (w + 1) T / W), so a unit is cut where a worker's run ends.  A piece
-// is the overlap of unit u and worker w; u + w grows strictly from piece to
-// piece, so it numbers the pieces' slots for partials, with no table of them.
-struct Group {
-  int64_t tile0;                // first tile
-  int32_t b0, n, table, prefix; // members b0 .. b0 + n - 1; table row that serves; tokens shared
-  int32_t unit0, pad;           // first unit
-};
-struct Seq {
-  int64_t tile0;
-  int32_t from, ctx, group, pad;  // own tokens from .. ctx - 1; its group or -1
-};
-struct Totals {
-  int64_t prefix_tiles, tiles, workers;
-};
-
-struct Params {
-  void* out;
-  float* lse;  // [B, H]
-  const void *q, *k, *v;
-  const int32_t *block_tables, *context_lens, *group_starts, *prefix_lens;
-  int64_t B, NG, H, HKV, BS, NB, MB;
-  float qscale;     // scale * log2(e)
-  int32_t G;        // query heads per KV head
-  int32_t warps;    // warps of the attention launch
-  int32_t bs_shift; // log2(BS) if BS is a power of two, else -1
-  // workspace
-  Totals* totals;
-  Group* groups;
-  Seq* seqs;
-  float2* part_ml;  // (running max in log2 units, sum)
-  float* part_o;
-  int64_t own_row0; // first partial row of the sequences' own units
-  int32_t* dev_status;
-};
-
-__host__ __device__ __forceinline__ int32_t cdiv(int32_t a, int32_t b) { return (a + b - 1) / b; }
-
-// Worker w's first tile, and the worker of tile x, for T tiles over W workers.
-__device__ __forceinline__ int64_t first_tile(int64_t w, int64_t T, int64_t W) { return w * T / W; }
-__device__ __forceinline__ int64_t worker_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W - 1) / T; }
 
 // ---------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------
 
 constexpr int kPlanThreads = 1024;
-constexpr int kMinTiles = 2;  // tiles per worker when there are few
+constexpr int kMinTiles = 2;    // tiles per worker when there are few
+constexpr int kMinTcTiles = 1;  // of the tensor-memory kernel's
 
 // Exclusive scan of (a, b) over the block on top of the running totals `base`.
 struct Pair {
@@ -148,21 +100,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
       gp.n = e - a;
       gp.table = first;
       gp.prefix = live > 1 ? max(0, min(p.prefix_lens[g], least)) : 0;
+      gp.tc = p.tc_rows && gp.n * G >= p.tc_rows;
     }
   }
   __syncthreads();
-  Pair base = {0, 0};  // tiles and units so far
+  Pair base = {0, 0}, tc_base = {0, 0};  // tiles and units so far
   for (int32_t g0 = 0; g0 < groups; g0 += kPlanThreads) {
     const int32_t g = g0 + tid;
-    Pair x = {0, 0};
+    Pair x = {0, 0}, y = {0, 0};
     if (g < groups) {
-      x.b = (int64_t)HKV * cdiv(p.groups[g].n * G, ROWS);
-      x.a = x.b * cdiv(p.groups[g].prefix, KT);
+      const Group& gp = p.groups[g];
+      if (gp.tc) {
+        y.b = (int64_t)HKV * cdiv(gp.n * G, TC_ROWS);
+        y.a = y.b * cdiv(gp.prefix, TC_KT);
+      } else {
+        x.b = (int64_t)HKV * cdiv(gp.n * G, ROWS);
+        x.a = x.b * cdiv(gp.prefix, KT);
+      }
     }
     const Pair at = block_scan(x, sums, base);
+    const Pair tc_at = p.tc_rows ? block_scan(y, sums, tc_base) : Pair{0, 0};
     if (g < groups) {
-      p.groups[g].tile0 = at.a;
-      p.groups[g].unit0 = (int32_t)at.b;
+      Group& gp = p.groups[g];
+      gp.tile0[0] = at.a;
+      gp.tile0[1] = tc_at.a;
+      gp.unit0[0] = (int32_t)at.b;
+      gp.unit0[1] = (int32_t)tc_at.b;
     }
   }
   const int64_t prefix_tiles = base.a;
@@ -178,14 +141,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     const Pair at = block_scan(x, sums, base);
     if (b < B) {
-      p.seqs[b].tile0 = at.a;
+      p.seqs[b].tile0[0] = at.a;
       p.seqs[b].from = from;
       p.seqs[b].ctx = ctx;
     }
   }
   if (tid == 0)
     *p.totals = Totals{prefix_tiles, base.a,
-                       min((int64_t)p.warps, max((base.a + kMinTiles - 1) / kMinTiles, (int64_t)1))};
+                       min((int64_t)p.warps, max((base.a + kMinTiles - 1) / kMinTiles, (int64_t)1)), tc_base.a,
+                       min((int64_t)p.tc_ctas, max((tc_base.a + kMinTcTiles - 1) / kMinTcTiles, (int64_t)1))};
 }
 
 // ---------------------------------------------------------------------------
@@ -198,21 +162,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
 struct Item {
   int32_t table, b0, r0, nrows, kvh, t0, t1, prow;
 };
-
-// The last of n entries (their tile0 rising from at most x) with tile0 <= x.
-// All lanes probe at once: two steps for 1024 entries.
-template <typename E>
-__device__ __forceinline__ int32_t find(const E* e, int32_t n, int64_t x, int lane) {
-  int32_t lo = 0, len = n;  // the answer is in [lo, lo + len)
-  while (len > 1) {
-    const int32_t step = (len + 31) / 32, at = lo + lane * step;
-    const uint32_t m = __ballot_sync(0xffffffffu, lane * step < len && e[at].tile0 <= x);
-    const int32_t k = 31 - __clz(m);
-    len = min(step, len - k * step);
-    lo += k * step;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -275,10 +224,12 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const 
   constexpr int NST = C::STAGES, CH = D / 8;  // 16-byte chunks per row
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_wait();
+  // (with a tensor-memory launch before this one, the plan is complete when
+  // this grid starts: that launch waits for it before it lets this one go)
+  if (!p.tc_rows) pdl_wait();
   pdl_trigger();
   const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-  const Totals tot = *p.totals;
+  const Totals tot = load_plan(p.totals);
   // rows of a tile sit `D * 2` bytes apart with their 16-byte chunks permuted
   // by the row, so the eight rows of a matrix load fall on different banks
   auto chunk_at = [](int row, int c) -> uint32_t {
@@ -286,23 +237,25 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const 
   };
   // consecutive workers sit on different SMs
   const int64_t worker = warp * gridDim.x + blockIdx.x;
-  if (worker >= tot.workers) return;
   const int32_t HKV = (int32_t)p.HKV, own_y = cdiv(p.G, ROWS);
-  int64_t x = first_tile(worker, tot.tiles, tot.workers);
-  const int64_t end = first_tile(worker + 1, tot.tiles, tot.workers);
+  int64_t x = 0, end = 0;
+  if (worker < tot.workers) {
+    x = first_tile(worker, tot.tiles, tot.workers);
+    end = first_tile(worker + 1, tot.tiles, tot.workers);
+  }
   int32_t at = -1;  // the group or sequence of tile x; of which is `x < prefix_tiles`
   bool in_prefix = x < tot.prefix_tiles;
   if (x < end)
-    at = in_prefix ? find(p.groups, (int32_t)p.NG, x, lane) : find(p.seqs, (int32_t)p.B, x, lane);
+    at = in_prefix ? find<0>(p.groups, (int32_t)p.NG, x, lane) : find<0>(p.seqs, (int32_t)p.B, x, lane);
   while (x < end) {
     if (in_prefix && x >= tot.prefix_tiles) in_prefix = false, at = 0;
     Item im;
     int64_t left;  // tiles of the unit from x on
     if (in_prefix) {
-      const Group gp = p.groups[at];
+      const Group gp = load_plan(p.groups + at);
       const int32_t rows = gp.n * p.G, ry = cdiv(rows, ROWS), nt = cdiv(gp.prefix, KT);
-      const int64_t done = x - gp.tile0;
-      if (done >= (int64_t)HKV * ry * nt) { ++at; continue; }
+      const int64_t done = x - gp.tile0[0];
+      if (gp.tc || done >= (int64_t)HKV * ry * nt) { ++at; continue; }
       const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
       left = min((int64_t)(nt - j), end - x);
       im.table = gp.table;
@@ -312,11 +265,11 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const 
       im.nrows = min(ROWS, rows - im.r0);
       im.t0 = j * KT;
       im.t1 = min(gp.prefix, im.t0 + (int32_t)left * KT);
-      im.prow = (int32_t)((gp.unit0 + u + worker) * ROWS);
+      im.prow = (int32_t)((gp.unit0[0] + u + worker) * ROWS);
     } else {
-      const Seq sp = p.seqs[at];
+      const Seq sp = load_plan(p.seqs + at);
       const int32_t nt = cdiv(sp.ctx - sp.from, KT);
-      const int64_t done = x - sp.tile0;
+      const int64_t done = x - sp.tile0[0];
       if (done >= (int64_t)HKV * own_y * nt) { ++at; continue; }
       const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
       left = min((int64_t)(nt - j), end - x);
@@ -473,6 +426,8 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const 
       }
     }
   }
+  // the merge waits for this grid alone, so this grid ends after the one before
+  if (p.tc_rows) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -489,30 +444,35 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   const int64_t b = row / p.H;
   const int32_t h = (int32_t)(row % p.H), kv = h / p.G, g = h % p.G;
   const int32_t own_y = cdiv(p.G, ROWS), own_rows = min(p.G, ROWS);
-  const Totals tot = *p.totals;
-  const Seq sp = p.seqs[b];
-  // this row's pieces: slot0 + c * step, first of its prefix unit, then of its own
+  const Totals tot = load_plan(p.totals);
+  const Seq sp = load_plan(p.seqs + b);
+  // this row's pieces: first of its prefix unit, pre_step rows apart, then of its own
   int64_t pre0 = 0, own0 = 0;
-  int32_t n_pre = 0, n_own = 0;
+  int32_t n_pre = 0, n_own = 0, pre_step = 0;
   if (sp.group >= 0 && sp.from > 0) {
-    const Group gp = p.groups[sp.group];
-    const int32_t rows = gp.n * p.G, ry = cdiv(rows, ROWS), nt = cdiv(gp.prefix, KT);
-    const int32_t r = ((int32_t)b - gp.b0) * p.G + g, u = kv * ry + r / ROWS;
-    const int64_t a = gp.tile0 + (int64_t)u * nt;
-    const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
-    n_pre = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
-    pre0 = (gp.unit0 + u + w0) * ROWS + r % ROWS;
+    const Group gp = load_plan(p.groups + sp.group);
+    const int32_t rows = gp.n * p.G, r = ((int32_t)b - gp.b0) * p.G + g;
+    const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R), nt = cdiv(gp.prefix, gp.tc ? TC_KT : KT);
+    const int64_t tiles = gp.tc ? tot.tc_tiles : tot.tiles, workers = gp.tc ? tot.tc_workers : tot.workers;
+    const int32_t u = kv * ry + r / R;
+    const int64_t a = gp.tile0[gp.tc] + (int64_t)u * nt;
+    const int64_t w0 = worker_of(a, tiles, workers);
+    n_pre = (int32_t)(worker_of(a + nt - 1, tiles, workers) - w0) + 1;
+    pre0 = (gp.tc ? p.tc_row0 : 0) + (gp.unit0[gp.tc] + u + w0) * R + r % R;
+    pre_step = R;
+    // a unit of at most 128 rows: a piece from each chain
+    if (gp.tc && rows - r / R * R <= R / 2) pre_step = R / 2, n_pre *= 2;
   }
   if (sp.ctx > sp.from) {
     const int32_t nt = cdiv(sp.ctx - sp.from, KT), u = kv * own_y + g / ROWS;
-    const int64_t a = sp.tile0 + (int64_t)u * nt;
+    const int64_t a = sp.tile0[0] + (int64_t)u * nt;
     const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
     n_own = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
     own0 = p.own_row0 + (b * p.HKV * own_y + u + w0) * own_rows + g % ROWS;
   }
   const int n = n_pre + n_own;
   auto piece = [&](int c) -> int64_t {
-    return c < n_pre ? pre0 + (int64_t)c * ROWS : own0 + (int64_t)(c - n_pre) * own_rows;
+    return c < n_pre ? pre0 + (int64_t)c * pre_step : own0 + (int64_t)(c - n_pre) * own_rows;
   };
   float M = -INFINITY;
   for (int c = lane; c < n; c += 32) M = fmaxf(M, p.part_ml[piece(c)].x);
@@ -523,6 +483,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   for (int c = 0; c < n; ++c) {
     const int64_t at = piece(c);
     const float2 ml = p.part_ml[at];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a piece without keys, or only scores of -inf
     const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
     L = fmaf(w, ml.y, L);
 #pragma unroll
@@ -540,8 +501,11 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 // host
 // ---------------------------------------------------------------------------
 
+// Rows of a group from which the tensor-memory kernel takes its prefix.
+constexpr int kTcRows = 64;
+
 struct Layout {
-  int64_t own_row0;
+  int64_t own_row0, tc_row0;
   size_t groups, seqs, ml, o, total;
 };
 
@@ -550,12 +514,16 @@ static int warps_per_cta(int64_t D) {
 }
 
 // Slots for partials: unit + worker < units + workers, for prefixes with ROWS
-// rows each, for sequences' own units with min(G, ROWS).
+// rows each, for sequences' own units with min(G, ROWS), for the
+// tensor-memory kernel's with TC_ROWS.
 static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, Layout* y) {
   const int64_t G = H / HKV, warps = (int64_t)sms * warps_per_cta(D);
   const int64_t pre_units = NG ? HKV * (B * G / ROWS + NG) : 0, own_units = B * HKV * ((G + ROWS - 1) / ROWS);
   y->own_row0 = NG ? (pre_units + warps) * ROWS : 0;
-  const int64_t rows = y->own_row0 + (own_units + warps) * std::min<int64_t>(G, ROWS);
+  y->tc_row0 = y->own_row0 + (own_units + warps) * std::min<int64_t>(G, ROWS);
+  int64_t rows = y->tc_row0;
+  if (NG && B * G >= kTcRows && (D == 64 || D == 128))
+    rows += (HKV * (B * G / TC_ROWS + std::min<int64_t>(NG, B * G / kTcRows)) + sms) * TC_ROWS;
   if (rows >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   y->groups = 256;
@@ -564,21 +532,6 @@ static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int 
   y->o = y->ml + up((size_t)rows * sizeof(float2));
   y->total = y->o + up((size_t)rows * D * sizeof(float));
   return PA_OK;
-}
-
-template <typename K>
-static cudaError_t launch_pdl(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Params& p) {
-  cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 template <typename T, int D>
@@ -599,8 +552,13 @@ static int launch_typed(Params& p, int sms, cudaStream_t s) {
     }
   }
   p.warps = sms * C::WARPS;
+  p.tc_ctas = sms;
   plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
   e = cudaGetLastError();
+  if (e == cudaSuccess && p.tc_rows) {
+    const int st = launch_tc(p, DTypeId<T>::value, D, s);
+    if (st) return st;
+  }
   if (e == cudaSuccess) e = launch_pdl(kern, dim3((unsigned)sms), dim3(C::WARPS * 32), C::SMEM, s, p);
   if (e == cudaSuccess)
     e = launch_pdl(merge_kernel<T, D>, dim3((unsigned)((p.B * p.H + 7) / 8)), dim3(256), 0, s, p);
@@ -660,6 +618,7 @@ extern "C" int pa_paged_attention_shared(
   if (io_dtype != kv_dtype) return PA_ERR_DTYPE;
   if (block_size <= 0 || num_blocks < 0 || max_blocks < 0) return PA_ERR_INVALID_ARGUMENT;
   if (num_seqs == 0) return PA_OK;
+  if (num_blocks == 0) return PA_ERR_INVALID_ARGUMENT;
   if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens ||
       (num_groups && (!group_starts || !prefix_lens)))
     return PA_ERR_INVALID_ARGUMENT;
@@ -703,6 +662,9 @@ extern "C" int pa_paged_attention_shared(
   p.groups = reinterpret_cast<shared::Group*>(ws + y.groups);
   p.seqs = reinterpret_cast<shared::Seq*>(ws + y.seqs);
   p.own_row0 = y.own_row0;
+  p.tc_row0 = y.tc_row0;
+  if (num_groups && num_seqs * p.G >= shared::kTcRows && shared::tc_takes(head_dim, block_size, num_blocks))
+    p.tc_rows = shared::kTcRows;
   p.part_ml = reinterpret_cast<float2*>(ws + y.ml);
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.dev_status = dev_status;
