@@ -9,11 +9,11 @@
 // rows of one product, and each K/V element of the prefix is read once a group
 // instead of once a sequence.
 //
-// Launches, chained with programmatic dependent launch: a plan (one CTA: the
-// groups' usable prefixes and running counts of the work), the prefixes of
-// groups with many rows on the tensor cores (shared_tc.cu), all other prefixes
-// and the sequences' own tokens (every warp takes an equal run of the work),
-// and the merge of the partials.
+// Two launches, the second a programmatic dependent of the first: the attention
+// and the merge of its partials.  Every CTA of the first makes the same plan in
+// shared memory (the groups' usable prefixes, running counts of the work) and
+// takes an equal run of the work; only for many sequences the plan is a launch
+// of its own.
 #include <algorithm>
 #include <mutex>
 #include <vector>
@@ -23,411 +23,31 @@
 namespace pa {
 namespace shared {
 
-// ---------------------------------------------------------------------------
-// plan
-// ---------------------------------------------------------------------------
-
-constexpr int kPlanThreads = 1024;
-constexpr int kMinTiles = 2;    // tiles per worker when there are few
-constexpr int kMinTcTiles = 1;  // of the tensor-memory kernel's
-
-// Exclusive scan of (a, b) over the block on top of the running totals `base`.
-struct Pair {
-  int64_t a, b;
-};
-__device__ __forceinline__ Pair block_scan(Pair x, Pair* warp_sums, Pair& base) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto warp_scan = [&](Pair s) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o);
-      if (lane >= o) s.a += a, s.b += b;
-    }
-    return s;
-  };
-  const Pair s = warp_scan(x);
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = s;
-  __syncthreads();
-  if (warp == 0) warp_sums[lane] = warp_scan(warp_sums[lane]);
-  __syncthreads();
-  const Pair before = warp ? warp_sums[warp - 1] : Pair{0, 0};
-  const Pair r = {base.a + before.a + s.a - x.a, base.b + before.b + s.b - x.b};
-  base.a += warp_sums[31].a;
-  base.b += warp_sums[31].b;
-  return r;
-}
-
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ Params p) {
-  __shared__ Pair sums[32];
+// The plan as a launch of its own, for more sequences or groups than kPlanMax.
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
-  const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
-  const int32_t own_y = cdiv(G, ROWS);
-  auto context = [&](int32_t b) {
-    const int32_t c = p.context_lens[b];
-    if (c > max_ctx) report(p.dev_status, PA_DEVERR_CONTEXT);
-    return min(max(c, 0), max_ctx);
-  };
-  // group bounds that are not 0 <= s_0 <= s_1 <= ... <= B: no sharing at all
-  int bad = 0;
-  for (int32_t g = tid; g < NG; g += kPlanThreads) {
-    const int32_t a = p.group_starts[g], b = p.group_starts[g + 1];
-    bad |= a < 0 || b < a || b > B;
-  }
-  bad = __syncthreads_or(bad);
-  if (bad && tid == 0) report(p.dev_status, PA_DEVERR_GROUP);
-  const int32_t groups = bad ? 0 : NG;
-  for (int32_t b = tid; b < B; b += kPlanThreads) p.seqs[b].group = -1;
-  __syncthreads();
-  // a group's usable prefix: no longer than any member that has tokens; the
-  // first such member's table row serves it.  One member alone shares nothing.
-  for (int32_t g = warp; g < groups; g += kPlanThreads / 32) {
-    const int32_t a = p.group_starts[g], e = p.group_starts[g + 1];
-    int32_t least = 0x7fffffff, first = 0x7fffffff, live = 0;
-    for (int32_t b = a + lane; b < e; b += 32) {
-      const int32_t c = context(b);
-      if (c > 0) least = min(least, c), first = min(first, b), ++live;
-      p.seqs[b].group = g;
-    }
-    least = __reduce_min_sync(0xffffffffu, least);
-    first = __reduce_min_sync(0xffffffffu, first);
-    live = __reduce_add_sync(0xffffffffu, live);
-    if (lane == 0) {
-      Group& gp = p.groups[g];
-      gp.b0 = a;
-      gp.n = e - a;
-      gp.table = first;
-      gp.prefix = live > 1 ? max(0, min(p.prefix_lens[g], least)) : 0;
-      gp.tc = p.tc_rows && gp.n * G >= p.tc_rows;
-    }
-  }
-  __syncthreads();
-  Pair base = {0, 0}, tc_base = {0, 0};  // tiles and units so far
-  for (int32_t g0 = 0; g0 < groups; g0 += kPlanThreads) {
-    const int32_t g = g0 + tid;
-    Pair x = {0, 0}, y = {0, 0};
-    if (g < groups) {
-      const Group& gp = p.groups[g];
-      if (gp.tc) {
-        y.b = (int64_t)HKV * cdiv(gp.n * G, TC_ROWS);
-        y.a = y.b * cdiv(gp.prefix, TC_KT);
-      } else {
-        x.b = (int64_t)HKV * cdiv(gp.n * G, ROWS);
-        x.a = x.b * cdiv(gp.prefix, KT);
-      }
-    }
-    const Pair at = block_scan(x, sums, base);
-    const Pair tc_at = p.tc_rows ? block_scan(y, sums, tc_base) : Pair{0, 0};
-    if (g < groups) {
-      Group& gp = p.groups[g];
-      gp.tile0[0] = at.a;
-      gp.tile0[1] = tc_at.a;
-      gp.unit0[0] = (int32_t)at.b;
-      gp.unit0[1] = (int32_t)tc_at.b;
-    }
-  }
-  const int64_t prefix_tiles = base.a;
-  for (int32_t b0 = 0; b0 < B; b0 += kPlanThreads) {
-    const int32_t b = b0 + tid;
-    Pair x = {0, 0};
-    int32_t ctx = 0, from = 0;
-    if (b < B) {
-      const int32_t g = p.seqs[b].group;
-      ctx = context(b);
-      if (g >= 0) from = min(p.groups[g].prefix, ctx);
-      x.a = (int64_t)HKV * own_y * cdiv(ctx - from, KT);
-    }
-    const Pair at = block_scan(x, sums, base);
-    if (b < B) {
-      p.seqs[b].tile0[0] = at.a;
-      p.seqs[b].from = from;
-      p.seqs[b].ctx = ctx;
-    }
-  }
-  if (tid == 0)
-    *p.totals = Totals{prefix_tiles, base.a,
-                       min((int64_t)p.warps, max((base.a + kMinTiles - 1) / kMinTiles, (int64_t)1)), tc_base.a,
-                       min((int64_t)p.tc_ctas, max((tc_base.a + kMinTcTiles - 1) / kMinTcTiles, (int64_t)1))};
+  make_plan(p, plan_at(p, 0), reinterpret_cast<int32_t*>(p.plan + p.scratch_off), true);
 }
 
-// ---------------------------------------------------------------------------
-// attention: one warp per worker
-// ---------------------------------------------------------------------------
-
-// What a warp computes at a time: rows r0 .. r0 + nrows - 1 of a unit (row r:
-// sequence b0 + r / G, head kvh * G + r % G) against keys t0 .. t1 - 1 of table
-// row `table`; partials from row prow on.
-struct Item {
-  int32_t table, b0, r0, nrows, kvh, t0, t1, prow;
-};
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// c[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half*) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-               "{%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16*) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-               "{%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16*) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half*) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
+// All of the work by warps: pools that the tensor-memory part does not load.
 template <int D> struct Cfg {
   static constexpr int STAGES = 4;
-  static constexpr int STAGE = 2 * KT * D * 2;  // K tile, V tile
-  static constexpr int WARP = STAGES * STAGE;
-  // warps per CTA (one CTA per SM): what 224 KB of stages hold, 16 at most
-  static constexpr int WARPS = 224 * 1024 / WARP < 16 ? 224 * 1024 / WARP : 16;
-  static constexpr int SMEM = WARPS * WARP;
+  static constexpr int RING = STAGES * (int)stage_bytes(D);
+  // warps per CTA (one CTA per SM): what 224 KB of rings hold, 16 at most
+  static constexpr int WARPS = 224 * 1024 / RING < 16 ? 224 * 1024 / RING : 16;
+  static constexpr int SMEM = WARPS * RING;
+  static_assert(plan_scratch(kPlanMax, kPlanMax) <= SMEM, "the plan's scratch is in the rings");
 };
 
-// A warp streams its item's K and V rows through a ring of its own (16-byte
-// asynchronous copies, so any page size and any first token serve), with the
-// keys of a tile as the N of S = Q K^T and the K of P V; the running maximum
-// and sum, the products' sums and O stay in fp32 registers.  P is rounded to
-// the pool's type for the second product (its error, 2^-9 or 2^-12 of a weight
-// at most and averaged over the keys, is at the level of the output's own
-// rounding); the sum l is of the unrounded weights.
 template <typename T, int D>
-__global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<D>;
-  constexpr int NST = C::STAGES, CH = D / 8;  // 16-byte chunks per row
+__global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) warps_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // (with a tensor-memory launch before this one, the plan is complete when
-  // this grid starts: that launch waits for it before it lets this one go)
-  if (!p.tc_rows) pdl_wait();
+  const int warp = threadIdx.x >> 5;
   pdl_trigger();
-  const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-  const Totals tot = load_plan(p.totals);
-  // rows of a tile sit `D * 2` bytes apart with their 16-byte chunks permuted
-  // by the row, so the eight rows of a matrix load fall on different banks
-  auto chunk_at = [](int row, int c) -> uint32_t {
-    return (uint32_t)(row * (D * 2) + ((c ^ (CH >= 8 ? (row & 7) : ((row >> 1) & 3))) << 4));
-  };
+  const Plan plan = take_plan(p, smem);
   // consecutive workers sit on different SMs
-  const int64_t worker = warp * gridDim.x + blockIdx.x;
-  const int32_t HKV = (int32_t)p.HKV, own_y = cdiv(p.G, ROWS);
-  int64_t x = 0, end = 0;
-  if (worker < tot.workers) {
-    x = first_tile(worker, tot.tiles, tot.workers);
-    end = first_tile(worker + 1, tot.tiles, tot.workers);
-  }
-  int32_t at = -1;  // the group or sequence of tile x; of which is `x < prefix_tiles`
-  bool in_prefix = x < tot.prefix_tiles;
-  if (x < end)
-    at = in_prefix ? find<0>(p.groups, (int32_t)p.NG, x, lane) : find<0>(p.seqs, (int32_t)p.B, x, lane);
-  while (x < end) {
-    if (in_prefix && x >= tot.prefix_tiles) in_prefix = false, at = 0;
-    Item im;
-    int64_t left;  // tiles of the unit from x on
-    if (in_prefix) {
-      const Group gp = load_plan(p.groups + at);
-      const int32_t rows = gp.n * p.G, ry = cdiv(rows, ROWS), nt = cdiv(gp.prefix, KT);
-      const int64_t done = x - gp.tile0[0];
-      if (gp.tc || done >= (int64_t)HKV * ry * nt) { ++at; continue; }
-      const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
-      left = min((int64_t)(nt - j), end - x);
-      im.table = gp.table;
-      im.b0 = gp.b0;
-      im.kvh = u / ry;
-      im.r0 = (u - im.kvh * ry) * ROWS;
-      im.nrows = min(ROWS, rows - im.r0);
-      im.t0 = j * KT;
-      im.t1 = min(gp.prefix, im.t0 + (int32_t)left * KT);
-      im.prow = (int32_t)((gp.unit0[0] + u + worker) * ROWS);
-    } else {
-      const Seq sp = load_plan(p.seqs + at);
-      const int32_t nt = cdiv(sp.ctx - sp.from, KT);
-      const int64_t done = x - sp.tile0[0];
-      if (done >= (int64_t)HKV * own_y * nt) { ++at; continue; }
-      const int32_t u = (int32_t)(done / nt), j = (int32_t)(done - (int64_t)u * nt);
-      left = min((int64_t)(nt - j), end - x);
-      im.table = im.b0 = at;
-      im.kvh = u / own_y;
-      im.r0 = (u - im.kvh * own_y) * ROWS;
-      im.nrows = min(ROWS, p.G - im.r0);
-      im.t0 = sp.from + j * KT;
-      im.t1 = min(sp.ctx, im.t0 + (int32_t)left * KT);
-      im.prow = (int32_t)(p.own_row0 + ((int64_t)at * HKV * own_y + u + worker) * min(p.G, ROWS));
-    }
-    x += left;
-    const int32_t* table = p.block_tables + (int64_t)im.table * p.MB;
-    const int n_tiles = (im.t1 - im.t0 + KT - 1) / KT;
-
-    // pool row (in rows of D elements) of token t0 + 16 j + lane, lanes 0-15
-    auto row_of = [&](int j) -> uint32_t {
-      const int32_t t = im.t0 + j * KT + lane;
-      if (lane >= KT || t >= im.t1) return 0xffffffffu;
-      const int32_t page = p.bs_shift >= 0 ? t >> p.bs_shift : t / (int32_t)p.BS;
-      int32_t blk = __ldg(table + page);
-      if (blk < 0 || blk >= p.NB) {
-        report(p.dev_status, PA_DEVERR_BLOCK_ID);
-        blk = 0;
-      }
-      return (uint32_t)(((int64_t)blk * p.BS + (t - page * (int32_t)p.BS)) * p.HKV + im.kvh);
-    };
-    // rows past the item's last key are zeros: their scores are masked, and
-    // no weight of zero meets a NaN of an unwritten row
-    auto load = [&](int j, uint32_t row) {
-      if (j < n_tiles) {
-        const uint32_t st = ring + (j % NST) * C::STAGE;
-#pragma unroll
-        for (int i = 0; i < KT * CH / 32; ++i) {
-          const int idx = i * 32 + lane, r = idx / CH, c = idx % CH;
-          const uint32_t pr = __shfl_sync(0xffffffffu, row, r);
-          const int bytes = pr == 0xffffffffu ? 0 : 16;
-          const int64_t off = bytes ? ((int64_t)pr * CH + c) * 16 : 0;
-          cp_async16(st + chunk_at(r, c), static_cast<const char*>(p.k) + off, bytes);
-          cp_async16(st + KT * D * 2 + chunk_at(r, c), static_cast<const char*>(p.v) + off, bytes);
-        }
-      }
-      cp_async_commit();
-    };
-
-    uint32_t rows_next = row_of(0);
-#pragma unroll
-    for (int j = 0; j < NST - 1; ++j) {
-      const uint32_t rows = rows_next;
-      rows_next = row_of(j + 1);
-      load(j, rows);
-    }
-
-    // Q: lane holds rows lane / 4 and lane / 4 + 8 of the A operand
-    uint32_t qa[D / 16][4];
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = im.r0 + (lane >> 2) + 8 * hf;
-      const bool in = (lane >> 2) + 8 * hf < im.nrows;
-      const T* src = static_cast<const T*>(p.q) +
-                     ((int64_t)(im.b0 + r / p.G) * p.H + im.kvh * p.G + r % p.G) * D + 2 * (lane & 3);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        qa[kk][hf] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
-        qa[kk][hf + 2] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
-      }
-    }
-
-    float o[D / 8][4];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const int mi = lane >> 3, mr = lane & 7;  // matrix and row this lane addresses
-
-    for (int j = 0; j < n_tiles; ++j) {
-      const uint32_t rows = rows_next;
-      rows_next = row_of(j + NST);
-      cp_async_wait<NST - 2>();
-      __syncwarp();
-      load(j + NST - 1, rows);  // into the stage of tile j - 1, which every lane has left
-      const uint32_t ks = ring + (j % NST) * C::STAGE, vs = ks + KT * D * 2;
-      float s[2][4] = {};
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b[4];
-        ldsm4(b, ks + chunk_at(mr + 8 * (mi >> 1), 2 * kk + (mi & 1)));
-        mma(s[0], qa[kk], b[0], b[1], (T*)nullptr);
-        mma(s[1], qa[kk], b[2], b[3], (T*)nullptr);
-      }
-      const int valid = im.t1 - im.t0 - j * KT;
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = 8 * n + 2 * (lane & 3) + (e & 1) < valid;
-          s[n][e] = in ? s[n][e] * p.qscale : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-        }
-      float alpha[2], base[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
-        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
-        const float mn = fmaxf(m[hf], mx[hf]);
-        base[hf] = mn == -INFINITY ? 0.f : mn;  // only -inf scores so far
-        alpha[hf] = fast_exp2(m[hf] - base[hf]);
-        m[hf] = mn;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= alpha[0];
-          o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1];
-          o[i][3] *= alpha[1];
-        }
-        l[0] *= alpha[0];
-        l[1] *= alpha[1];
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = fast_exp2(s[n][e] - base[e >> 1]);
-          l[e >> 1] += s[n][e];
-        }
-      const uint32_t pa[4] = {pack2(s[0][0], s[0][1], (T*)nullptr), pack2(s[0][2], s[0][3], (T*)nullptr),
-                              pack2(s[1][0], s[1][1], (T*)nullptr), pack2(s[1][2], s[1][3], (T*)nullptr)};
-#pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        uint32_t b[4];
-        ldsm4t(b, vs + chunk_at(mr + 8 * (mi & 1), 2 * dd + (mi >> 1)));
-        mma(o[2 * dd], pa, b[0], b[1], (T*)nullptr);
-        mma(o[2 * dd + 1], pa, b[2], b[3], (T*)nullptr);
-      }
-      __syncwarp();
-    }
-    cp_async_wait<0>();
-    __syncwarp();
-
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-      const int r = (lane >> 2) + 8 * hf;
-      if (r < im.nrows) {
-        const int64_t row = im.prow + r;
-        if ((lane & 3) == 0) p.part_ml[row] = make_float2(m[hf], l[hf]);
-        float* dst = p.part_o + row * D + 2 * (lane & 3);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
-      }
-    }
-  }
-  // the merge waits for this grid alone, so this grid ends after the one before
-  if (p.tc_rows) pdl_wait();
+  warp_work<T, D, Cfg<D>::STAGES>(p, plan, load_plan(plan.totals), smem_u32(smem) + warp * Cfg<D>::RING,
+                                  (int64_t)warp * gridDim.x + blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -444,21 +64,22 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   const int64_t b = row / p.H;
   const int32_t h = (int32_t)(row % p.H), kv = h / p.G, g = h % p.G;
   const int32_t own_y = cdiv(p.G, ROWS), own_rows = min(p.G, ROWS);
-  const Totals tot = load_plan(p.totals);
-  const Seq sp = load_plan(p.seqs + b);
+  const Plan plan = plan_at(p, 0);
+  const Totals tot = load_plan(plan.totals);
+  const Seq sp = load_plan(plan.seqs + b);
   // this row's pieces: first of its prefix unit, pre_step rows apart, then of its own
   int64_t pre0 = 0, own0 = 0;
   int32_t n_pre = 0, n_own = 0, pre_step = 0;
   if (sp.group >= 0 && sp.from > 0) {
-    const Group gp = load_plan(p.groups + sp.group);
+    const Group gp = load_plan(plan.groups + sp.group);
     const int32_t rows = gp.n * p.G, r = ((int32_t)b - gp.b0) * p.G + g;
     const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R), nt = cdiv(gp.prefix, gp.tc ? TC_KT : KT);
     const int64_t tiles = gp.tc ? tot.tc_tiles : tot.tiles, workers = gp.tc ? tot.tc_workers : tot.workers;
     const int32_t u = kv * ry + r / R;
-    const int64_t a = gp.tile0[gp.tc] + (int64_t)u * nt;
+    const int64_t a = (gp.tc ? gp.tile0[1] : gp.tile0[0]) + (int64_t)u * nt;
     const int64_t w0 = worker_of(a, tiles, workers);
     n_pre = (int32_t)(worker_of(a + nt - 1, tiles, workers) - w0) + 1;
-    pre0 = (gp.tc ? p.tc_row0 : 0) + (gp.unit0[gp.tc] + u + w0) * R + r % R;
+    pre0 = (gp.tc ? p.tc_row0 : 0) + ((gp.tc ? gp.unit0[1] : gp.unit0[0]) + u + w0) * R + r % R;
     pre_step = R;
     // a unit of at most 128 rows: a piece from each chain
     if (gp.tc && rows - r / R * R <= R / 2) pre_step = R / 2, n_pre *= 2;
@@ -474,26 +95,63 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   auto piece = [&](int c) -> int64_t {
     return c < n_pre ? pre0 + (int64_t)c * pre_step : own0 + (int64_t)(c - n_pre) * own_rows;
   };
-  float M = -INFINITY;
-  for (int c = lane; c < n; c += 32) M = fmaxf(M, p.part_ml[piece(c)].x);
+  // 32 pieces at a time, lane c with the maximum and sum of piece c; then their
+  // O, several in flight
+  constexpr int V = D >= 128 ? 4 : D / 32;  // elements per load
+  float acc[E] = {}, L = 0.f, M = -INFINITY;
+  for (int c0 = 0; c0 < n; c0 += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (c0 + lane < n) ml = p.part_ml[piece(c0 + lane)];
+    const bool none = ml.x == -INFINITY && ml.y == 0.f;  // without keys, or only scores of -inf: O not read
+    float top = ml.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float acc[E] = {}, L = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < n; ++c) {
-    const int64_t at = piece(c);
-    const float2 ml = p.part_ml[at];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a piece without keys, or only scores of -inf
-    const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-    L = fmaf(w, ml.y, L);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float Mn = fmaxf(M, top), base = Mn == -INFINITY ? 0.f : Mn;
+    const float alpha = fast_exp2(M - base), w = fast_exp2(ml.x - base);
+    M = Mn;
+    float l = none ? 0.f : w * ml.y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(w, p.part_o[at * D + e * 32 + lane], acc[e]);
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    L = fmaf(L, alpha, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= alpha;
+    const uint32_t read = __ballot_sync(0xffffffffu, !none);
+#pragma unroll 8
+    for (int c = 0; c < min(32, n - c0); ++c) {
+      const float wc = __shfl_sync(0xffffffffu, w, c);
+      const float* src = p.part_o + piece(c0 + c) * D + lane * V;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = 0.f;
+      if (read >> c & 1)
+#pragma unroll
+        for (int i = 0; i < E / V; ++i) {
+          if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
+            x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
+          } else if constexpr (V == 2) {
+            const float2 f = *reinterpret_cast<const float2*>(src);
+            x[0] = f.x, x[1] = f.y;
+          } else {
+            x[0] = *src;
+          }
+        }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(wc, x[e], acc[e]);
+    }
   }
   // no key, or only scores of -inf: L = 0, so out is NaN and lse -inf
   const float inv = 1.f / L;
-  T* out = static_cast<T*>(p.out) + row * D;
+  T* out = static_cast<T*>(p.out) + row * D + lane * V;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e * 32 + lane] = T(acc[e] * inv);
+  for (int i = 0; i < E / V; ++i) {
+    struct alignas(2 * V) {
+      T x[V];
+    } v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v.x[e] = T(acc[i * V + e] * inv);
+    *reinterpret_cast<decltype(v)*>(out + i * 128) = v;
+  }
   if (p.lse && lane == 0) p.lse[row] = (M + log2f(L)) * kLn2;
 }
 
@@ -501,12 +159,13 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 // host
 // ---------------------------------------------------------------------------
 
-// Rows of a group from which the tensor-memory kernel takes its prefix.
-constexpr int kTcRows = 64;
+// Rows of a group from which its prefix may go to the tensor memory.
+constexpr int kTcRows = 33;
 
 struct Layout {
-  int64_t own_row0, tc_row0;
-  size_t groups, seqs, ml, o, total;
+  bool tc, planned;
+  int64_t warps, plan_bytes, group_off, seq_off, scratch_off, own_row0, tc_row0;
+  size_t ml, o, total;
 };
 
 static int warps_per_cta(int64_t D) {
@@ -514,59 +173,67 @@ static int warps_per_cta(int64_t D) {
 }
 
 // Slots for partials: unit + worker < units + workers, for prefixes with ROWS
-// rows each, for sequences' own units with min(G, ROWS), for the
-// tensor-memory kernel's with TC_ROWS.
-static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, Layout* y) {
-  const int64_t G = H / HKV, warps = (int64_t)sms * warps_per_cta(D);
+// rows each, for sequences' own units with min(G, ROWS), for the tensor
+// memory's with TC_ROWS.  `tc`: whether this launch has that part (a size query,
+// which does not know the pool, assumes the larger).
+static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, bool tc, Layout* y) {
+  const int64_t G = H / HKV;
+  y->tc = tc && NG && B * G >= kTcRows && (D == 64 || D == 128);
+  y->warps = (int64_t)sms * (y->tc ? kTcWarps : warps_per_cta(D));
+  const int64_t most = (int64_t)sms * std::max(kTcWarps, warps_per_cta(D));
   const int64_t pre_units = NG ? HKV * (B * G / ROWS + NG) : 0, own_units = B * HKV * ((G + ROWS - 1) / ROWS);
-  y->own_row0 = NG ? (pre_units + warps) * ROWS : 0;
-  y->tc_row0 = y->own_row0 + (own_units + warps) * std::min<int64_t>(G, ROWS);
+  y->own_row0 = NG ? (pre_units + most) * ROWS : 0;
+  y->tc_row0 = y->own_row0 + (own_units + most) * std::min<int64_t>(G, ROWS);
   int64_t rows = y->tc_row0;
-  if (NG && B * G >= kTcRows && (D == 64 || D == 128))
-    rows += (HKV * (B * G / TC_ROWS + std::min<int64_t>(NG, B * G / kTcRows)) + sms) * TC_ROWS;
-  if (rows >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  y->groups = 256;
-  y->seqs = y->groups + up((size_t)NG * sizeof(Group));
-  y->ml = y->seqs + up((size_t)B * sizeof(Seq));
-  y->o = y->ml + up((size_t)rows * sizeof(float2));
-  y->total = y->o + up((size_t)rows * D * sizeof(float));
+  if (y->tc) rows += (HKV * (B * G / TC_ROWS + std::min<int64_t>(NG, B * G / kTcRows)) + sms) * TC_ROWS;
+  if (rows >= (int64_t(1) << 31) || B * H >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
+  auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  y->planned = B > kPlanMax || NG > kPlanMax;
+  y->group_off = 256;
+  y->seq_off = y->group_off + up(NG * (int64_t)sizeof(Group));
+  y->scratch_off = y->seq_off + up(B * (int64_t)sizeof(Seq));
+  y->plan_bytes = y->scratch_off + (y->planned ? up(plan_scratch(B, NG)) : 0);
+  y->ml = (size_t)(y->plan_bytes * (y->planned ? 1 : sms));
+  y->o = y->ml + (size_t)up(rows * (int64_t)sizeof(float2));
+  y->total = y->o + (size_t)up(rows * D * (int64_t)sizeof(float));
   return PA_OK;
 }
 
 template <typename T, int D>
-static int launch_typed(Params& p, int sms, cudaStream_t s) {
-  using C = Cfg<D>;
-  auto kern = attention_kernel<T, D>;
-  static std::mutex mu;
-  static std::vector<int> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_status(e);
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    if (std::find(done.begin(), done.end(), dev) == done.end()) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-      if (e != cudaSuccess) return cuda_status(e);
-      done.push_back(dev);
-    }
+static int launch_typed(const Params& p, int sms, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (p.planned) {
+    plan_kernel<<<1, 1024, 0, s>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_status(e);
   }
-  p.warps = sms * C::WARPS;
-  p.tc_ctas = sms;
-  plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  e = cudaGetLastError();
-  if (e == cudaSuccess && p.tc_rows) {
+  if (p.tc_rows) {
     const int st = launch_tc(p, DTypeId<T>::value, D, s);
     if (st) return st;
+  } else {
+    using C = Cfg<D>;
+    auto kern = warps_kernel<T, D>;
+    static std::mutex mu;
+    static std::vector<int> done;
+    int dev = 0;
+    e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_status(e);
+    {
+      std::lock_guard<std::mutex> lk(mu);
+      if (std::find(done.begin(), done.end(), dev) == done.end()) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return cuda_status(e);
+        done.push_back(dev);
+      }
+    }
+    e = launch(kern, sms, C::WARPS * 32, C::SMEM, s, p, p.planned);
+    if (e != cudaSuccess) return cuda_status(e);
   }
-  if (e == cudaSuccess) e = launch_pdl(kern, dim3((unsigned)sms), dim3(C::WARPS * 32), C::SMEM, s, p);
-  if (e == cudaSuccess)
-    e = launch_pdl(merge_kernel<T, D>, dim3((unsigned)((p.B * p.H + 7) / 8)), dim3(256), 0, s, p);
-  return cuda_status(e);
+  return cuda_status(launch(merge_kernel<T, D>, (p.B * p.H + 7) / 8, 256, 0, s, p, true));
 }
 
 template <typename T>
-static int launch_dtype(Params& p, int64_t D, int sms, cudaStream_t s) {
+static int launch_dtype(const Params& p, int64_t D, int sms, cudaStream_t s) {
   switch (D) {
     case 32: return launch_typed<T, 32>(p, sms, s);
     case 64: return launch_typed<T, 64>(p, sms, s);
@@ -599,7 +266,7 @@ extern "C" int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, in
   int sms = 0;
   if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
   shared::Layout y;
-  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, &y);
+  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, true, &y);
   if (st) return st;
   *bytes = y.total;
   return PA_OK;
@@ -631,7 +298,8 @@ extern "C" int pa_paged_attention_shared(
   int sms = 0;
   if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
   shared::Layout y;
-  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, &y);
+  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms,
+                      shared::tc_takes(head_dim, block_size, num_blocks), &y);
   if (st) return st;
   if (!workspace || workspace_bytes < y.total) return PA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PA_ERR_ALIGNMENT;
@@ -658,13 +326,17 @@ extern "C" int pa_paged_attention_shared(
   p.bs_shift = -1;
   if ((block_size & (block_size - 1)) == 0)
     for (p.bs_shift = 0; (int64_t(1) << p.bs_shift) < block_size; ++p.bs_shift) {}
-  p.totals = reinterpret_cast<shared::Totals*>(ws);
-  p.groups = reinterpret_cast<shared::Group*>(ws + y.groups);
-  p.seqs = reinterpret_cast<shared::Seq*>(ws + y.seqs);
+  p.plan = ws;
+  p.plan_bytes = y.plan_bytes;
+  p.group_off = y.group_off;
+  p.seq_off = y.seq_off;
+  p.scratch_off = y.scratch_off;
+  p.planned = y.planned;
+  p.warps = (int32_t)y.warps;
   p.own_row0 = y.own_row0;
   p.tc_row0 = y.tc_row0;
-  if (num_groups && num_seqs * p.G >= shared::kTcRows && shared::tc_takes(head_dim, block_size, num_blocks))
-    p.tc_rows = shared::kTcRows;
+  p.tc_rows = y.tc ? shared::kTcRows : 0;
+  p.tc_ctas = sms;
   p.part_ml = reinterpret_cast<float2*>(ws + y.ml);
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.dev_status = dev_status;

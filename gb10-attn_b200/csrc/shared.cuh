@@ -1,6 +1,7 @@
 // shared.cuh -- what the launches of the shared-prefix decode have in common:
-// how its work is counted, cut and numbered (shared.cu has the plan, the warp
-// kernel and the merge, shared_tc.cu the tensor-memory kernel).
+// how its work is counted, cut and numbered, the plan, and a warp's part of the
+// work (shared.cu has the launch for pools that the tensor-memory part cannot
+// load, the merge and the entry points, shared_tc.cu the launch that has both).
 #pragma once
 
 #include "common.cuh"
@@ -11,7 +12,7 @@ namespace shared {
 constexpr int KT = 16;    // keys per tile
 constexpr int ROWS = 16;  // query rows per item (the M of one mma)
 
-// tensor-memory kernel: keys per tile, rows per unit (two chains of 128; a unit
+// tensor-memory part: keys per tile, rows per unit (two chains of 128; a unit
 // of at most 128 rows gives both chains the same rows and every other tile)
 constexpr int TC_KT = 128;
 constexpr int TC_ROWS = 256;
@@ -24,12 +25,13 @@ constexpr int TC_ROWS = 256;
 // [w T / W, (w + 1) T / W), so a unit is cut where a worker's run ends.  A piece
 // is the overlap of unit u and worker w; u + w grows strictly from piece to
 // piece, so it numbers the pieces' slots for partials, with no table of them.
-//   Groups with many rows are the tensor-memory kernel's (shared_tc.cu), with
-// tiles, units and workers of its own, numbered the same way.
+//   The prefixes of groups with many rows are done in tensor memory
+// (shared_tc.cu), with tiles, units and workers (CTAs) of their own, numbered
+// the same way.
 struct alignas(16) Group {
-  long long tile0[2];           // first tile: of the warps' work, of the tensor-memory kernel's
+  long long tile0[2];           // first tile: of the warps' work, of the tensor memory's
   int32_t b0, n, table, prefix; // members b0 .. b0 + n - 1; table row that serves; tokens shared
-  int32_t unit0[2], tc, pad;    // first unit; whether the tensor-memory kernel does it
+  int32_t unit0[2], tc, pad;    // first unit; whether it is done in tensor memory
 };
 struct alignas(16) Seq {
   long long tile0[1];
@@ -37,7 +39,7 @@ struct alignas(16) Seq {
 };
 struct alignas(16) Totals {
   int64_t prefix_tiles, tiles, workers;  // the warps' work
-  int64_t tc_tiles, tc_workers;          // the tensor-memory kernel's
+  int64_t tc_tiles, tc_workers;          // the tensor memory's
 };
 
 struct Params {
@@ -48,17 +50,18 @@ struct Params {
   int64_t B, NG, H, HKV, BS, NB, MB;
   float qscale;     // scale * log2(e)
   int32_t G;        // query heads per KV head
-  int32_t warps;    // warps of the attention launch
+  int32_t warps;    // warps of the attention launch that take work
   int32_t bs_shift; // log2(BS) if BS is a power of two, else -1
   // workspace
-  Totals* totals;
-  Group* groups;
-  Seq* seqs;
+  char* plan;           // the plan (Plan below); every CTA that makes its own has one
+  int64_t plan_bytes;   // bytes of one
+  int64_t group_off, seq_off, scratch_off;  // its groups, sequences, scratch (made by plan_kernel only)
+  int32_t planned;      // a launch of its own makes the plan
   float2* part_ml;  // (running max in log2 units, sum)
   float* part_o;
   int64_t own_row0; // first partial row of the sequences' own units
-  int64_t tc_row0;  // and of the tensor-memory kernel's units
-  int32_t tc_rows;  // rows from which a group is the tensor-memory kernel's (0: none is)
+  int64_t tc_row0;  // and of the tensor memory's units
+  int32_t tc_rows;  // rows from which a group's prefix goes to the tensor memory (0: none does)
   int32_t tc_ctas;
   int32_t* dev_status;
 };
@@ -69,8 +72,7 @@ __host__ __device__ __forceinline__ int32_t cdiv(int32_t a, int32_t b) { return 
 __device__ __forceinline__ int64_t first_tile(int64_t w, int64_t T, int64_t W) { return w * T / W; }
 __device__ __forceinline__ int64_t worker_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W - 1) / T; }
 
-// One of the structs above, past the L1: the launch after next reads the plan
-// without having waited for it itself.
+// One of the structs above, in 16-byte loads.
 template <typename E> __device__ __forceinline__ E load_plan(const E* e) {
   static_assert(sizeof(E) % 16 == 0, "");
   union {
@@ -78,7 +80,7 @@ template <typename E> __device__ __forceinline__ E load_plan(const E* e) {
     E e;
   } u;
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(E) / 16; ++i) u.w[i] = __ldcg(reinterpret_cast<const int4*>(e) + i);
+  for (int i = 0; i < (int)sizeof(E) / 16; ++i) u.w[i] = reinterpret_cast<const int4*>(e)[i];
   return u.e;
 }
 
@@ -89,7 +91,7 @@ __device__ __forceinline__ int32_t find(const E* e, int32_t n, int64_t x, int la
   int32_t lo = 0, len = n;  // the answer is in [lo, lo + len)
   while (len > 1) {
     const int32_t step = (len + 31) / 32, at = lo + lane * step;
-    const uint32_t m = __ballot_sync(0xffffffffu, lane * step < len && __ldcg(&e[at].tile0[I]) <= x);
+    const uint32_t m = __ballot_sync(0xffffffffu, lane * step < len && e[at].tile0[I] <= x);
     const int32_t k = 31 - __clz(m);
     len = min(step, len - k * step);
     lo += k * step;
@@ -97,23 +99,502 @@ __device__ __forceinline__ int32_t find(const E* e, int32_t n, int64_t x, int la
   return lo;
 }
 
+// ---------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------
+
+struct Plan {
+  Totals* totals;
+  Group* groups;
+  Seq* seqs;
+};
+__device__ __forceinline__ Plan plan_at(const Params& p, int64_t copy) {
+  char* base = p.plan + copy * p.plan_bytes;
+  return {reinterpret_cast<Totals*>(base), reinterpret_cast<Group*>(base + p.group_off),
+          reinterpret_cast<Seq*>(base + p.seq_off)};
+}
+
+// Sequences and groups up to which every CTA makes the plan itself, in shared
+// memory: one launch less, which small calls notice.
+constexpr int kPlanMax = 1024;
+__host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) { return (2 * B + 3 * (NG + 1)) * 4; }
+
+constexpr int kMinTiles = 2;    // 16-key tiles per warp when there are few
+constexpr int kTcMinTiles = 3;  // 128-key tiles per CTA below which the warps do all
+
+// Exclusive scan of N values over the block on top of the running totals `base`.
+template <int N> struct Sums {
+  long long v[N];
+};
+template <int N>
+__device__ __forceinline__ Sums<N> block_scan(const Sums<N>& x, Sums<N>* warp_sums, Sums<N>& base) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  auto warp_scan = [&](Sums<N> s) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const long long y = __shfl_up_sync(0xffffffffu, s.v[i], o);
+        if (lane >= o) s.v[i] += y;
+      }
+    return s;
+  };
+  const Sums<N> s = warp_scan(x);
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  Sums<N> r = {}, all = {};
+  for (int w = 0; w < warps; ++w)  // at most 32, the same words for all lanes
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (w < warp) r.v[i] += warp_sums[w].v[i];
+      all.v[i] += warp_sums[w].v[i];
+    }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r.v[i] += base.v[i] + s.v[i] - x.v[i];
+    base.v[i] += all.v[i];
+  }
+  return r;
+}
+
+// One CTA makes the plan; `scratch`: plan_scratch() bytes, in shared memory or
+// its own part of the workspace.  Ends with a barrier.
+__device__ __forceinline__ void make_plan(const Params& p, const Plan& out, int32_t* scratch, bool tell) {
+  __shared__ Sums<3> sums[32];
+  __shared__ unsigned long long tc_work;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
+  const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
+  int32_t *ctx = scratch, *grp = ctx + B, *gs = grp + B, *pre = gs + NG + 1, *lead = pre + NG + 1;
+  if (tid == 0) tc_work = 0;
+  int far = 0;
+  for (int32_t b = tid; b < B; b += threads) {
+    const int32_t c = p.context_lens[b];
+    far |= c > max_ctx;
+    ctx[b] = min(max(c, 0), max_ctx);
+    grp[b] = -1;
+  }
+  for (int32_t g = tid; g < NG; g += threads) pre[g] = p.prefix_lens[g];
+  for (int32_t g = tid; g <= NG && NG; g += threads) gs[g] = p.group_starts[g];
+  if (far && tell) report(p.dev_status, PA_DEVERR_CONTEXT);
+  __syncthreads();
+  // group bounds that are not 0 <= s_0 <= s_1 <= ... <= B: no sharing at all
+  int bad = 0;
+  for (int32_t g = tid; g < NG; g += threads) bad |= gs[g] < 0 || gs[g + 1] < gs[g] || gs[g + 1] > B;
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0 && tell) report(p.dev_status, PA_DEVERR_GROUP);
+  const int32_t groups = bad ? 0 : NG;
+  // a group's usable prefix: no longer than any member that has tokens; the
+  // first such member's table row serves it.  One member alone shares nothing.
+  for (int32_t g = warp; g < groups; g += threads / 32) {
+    const int32_t a = gs[g], e = gs[g + 1];
+    int32_t least = 0x7fffffff, first = 0x7fffffff, live = 0;
+    for (int32_t b = a + lane; b < e; b += 32) {
+      const int32_t c = ctx[b];
+      if (c > 0) least = min(least, c), first = min(first, b), ++live;
+      grp[b] = g;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    first = __reduce_min_sync(0xffffffffu, first);
+    live = __reduce_add_sync(0xffffffffu, live);
+    if (lane == 0) {
+      const int32_t prefix = live > 1 ? max(0, min(pre[g], least)) : 0;
+      pre[g] = prefix;
+      lead[g] = first;
+      if (p.tc_rows && (e - a) * G >= p.tc_rows)
+        atomicAdd(&tc_work, (unsigned long long)HKV * cdiv((e - a) * G, TC_ROWS) * cdiv(prefix, TC_KT));
+    }
+  }
+  __syncthreads();
+  const bool use_tc = p.tc_rows && tc_work >= (unsigned long long)kTcMinTiles * p.tc_ctas;
+  Sums<3> base = {};  // tiles of the warps and of the tensor memory, units (tensor memory's in the high half)
+  for (int32_t g0 = 0; g0 < groups; g0 += threads) {
+    const int32_t g = g0 + tid;
+    Sums<3> x = {};
+    int32_t n = 0, prefix = 0, tc = 0;
+    if (g < groups) {
+      n = gs[g + 1] - gs[g];
+      prefix = pre[g];
+      tc = use_tc && n * G >= p.tc_rows;
+      const long long units = (long long)HKV * cdiv(n * G, tc ? TC_ROWS : ROWS);
+      x = tc ? Sums<3>{{0, units * cdiv(prefix, TC_KT), units << 32}} : Sums<3>{{units * cdiv(prefix, KT), 0, units}};
+    }
+    const Sums<3> at = block_scan(x, sums, base);
+    if (g < groups)
+      out.groups[g] = Group{{at.v[0], at.v[1]}, gs[g], n, lead[g], prefix,
+                            {(int32_t)(at.v[2] & 0xffffffff), (int32_t)(at.v[2] >> 32)}, tc, 0};
+  }
+  Sums<1> own = {{base.v[0]}};
+  for (int32_t b0 = 0; b0 < B; b0 += threads) {
+    const int32_t b = b0 + tid;
+    Sums<1> x = {};
+    int32_t from = 0, g = -1;
+    if (b < B) {
+      g = grp[b];
+      if (g >= 0) from = min(pre[g], ctx[b]);
+      x.v[0] = (long long)HKV * cdiv(G, ROWS) * cdiv(ctx[b] - from, KT);
+    }
+    const Sums<1> at = block_scan(x, reinterpret_cast<Sums<1>*>(sums), own);
+    if (b < B) out.seqs[b] = Seq{{at.v[0]}, from, ctx[b], g, 0};
+  }
+  if (tid == 0)
+    *out.totals = Totals{base.v[0], own.v[0],
+                         min((int64_t)p.warps, max(((int64_t)own.v[0] + kMinTiles - 1) / kMinTiles, (int64_t)1)),
+                         base.v[1], min((int64_t)p.tc_ctas, max((int64_t)base.v[1], (int64_t)1))};
+  __syncthreads();
+}
+
+// The plan that this CTA works by.
+__device__ __forceinline__ Plan take_plan(const Params& p, void* smem_scratch) {
+  if (p.planned) {
+    pdl_wait();
+    return plan_at(p, 0);
+  }
+  const Plan plan = plan_at(p, blockIdx.x);
+  make_plan(p, plan, static_cast<int32_t*>(smem_scratch), blockIdx.x == 0);
+  return plan;
+}
+
+// ---------------------------------------------------------------------------
+// a warp's work: its run of 16-key tiles
+// ---------------------------------------------------------------------------
+
+// What a warp computes at a time: rows r0 .. r0 + nrows - 1 of a unit (row r:
+// sequence b0 + r / G, head kvh * G + r % G) against keys t0 .. t1 - 1 of table
+// row `table`; partials from row prow on.
+struct Item {
+  int32_t table, b0, r0, nrows, kvh, t0, t1;
+  int64_t prow;
+};
+
+// The items of a worker's run, in order.
+struct Run {
+  const Group* groups;
+  const Seq* seqs;
+  int64_t left, worker, slot;    // tiles left; partial row of the entry's unit 0
+  int32_t at, u, j, nt, units;   // entry (a group, or a sequence if !pre), unit and tile in it
+  int32_t table, b0, rows, from, to, unit_y;
+  bool pre;
+
+  __device__ __forceinline__ Run(const Params& p, const Plan& plan, const Totals& tot, int64_t w, int lane)
+      : groups(plan.groups), seqs(plan.seqs), left(0), worker(w) {
+    at = u = j = units = 0;
+    pre = false;
+    if (w >= tot.workers) return;
+    const int64_t x = first_tile(w, tot.tiles, tot.workers);
+    left = first_tile(w + 1, tot.tiles, tot.workers) - x;
+    if (left == 0) return;
+    pre = x < tot.prefix_tiles;
+    at = pre ? find<0>(groups, (int32_t)p.NG, x, lane) : find<0>(seqs, (int32_t)p.B, x, lane);
+    const int64_t done = x - entry(p);
+    u = (int32_t)(done / nt);
+    j = (int32_t)(done - (int64_t)u * nt);
+  }
+  // Takes up entry `at`; its first tile.
+  __device__ __forceinline__ int64_t entry(const Params& p) {
+    int64_t tile0;
+    if (pre) {
+      const Group gp = load_plan(groups + at);
+      tile0 = gp.tile0[0];
+      table = gp.table;
+      b0 = gp.b0;
+      rows = gp.n * p.G;
+      from = 0;
+      to = gp.tc ? 0 : gp.prefix;
+      slot = (int64_t)gp.unit0[0] * ROWS;
+    } else {
+      const Seq sp = load_plan(seqs + at);
+      tile0 = sp.tile0[0];
+      table = b0 = at;
+      rows = p.G;
+      from = sp.from;
+      to = sp.ctx;
+      slot = p.own_row0 + (int64_t)at * p.HKV * cdiv(p.G, ROWS) * min(p.G, ROWS);
+    }
+    nt = cdiv(to - from, KT);
+    unit_y = cdiv(rows, ROWS);
+    units = nt ? (int32_t)p.HKV * unit_y : 0;
+    return tile0;
+  }
+  __device__ __forceinline__ bool next(const Params& p, Item& im) {
+    if (left == 0) return false;
+    while (u == units) {  // (an entry with tiles follows, since some are left)
+      if (++at == p.NG && pre) pre = false, at = 0;
+      entry(p);
+      u = 0;
+    }
+    const int32_t n = (int32_t)min((int64_t)(nt - j), left);
+    im.table = table;
+    im.b0 = b0;
+    im.kvh = u / unit_y;
+    im.r0 = (u - im.kvh * unit_y) * ROWS;
+    im.nrows = min(ROWS, rows - im.r0);
+    im.t0 = from + j * KT;
+    im.t1 = min(to, im.t0 + n * KT);
+    im.prow = slot + (u + worker) * (pre ? ROWS : min(p.G, ROWS));
+    left -= n;
+    j += n;
+    if (j == nt) j = 0, ++u;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half*) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16*) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16*) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half*) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// One stage of a warp's ring: the K rows of a tile, then its V rows.
+__host__ __device__ constexpr uint32_t stage_bytes(int D) { return 2 * KT * D * 2; }
+
+// A warp streams its items through a ring of its own: for each the rows of Q,
+// then tile after tile the rows of K and V (16-byte asynchronous copies, so any
+// page size and any first token serve).  The copies run NST - 1 stages ahead
+// across items, and the block ids one stage further, so no item waits for its
+// first bytes: with a few tiles an item that wait was most of the time.
+//   The keys of a tile are the N of S = Q K^T and the K of P V; the running
+// maximum and sum, the products' sums and O stay in fp32 registers.  P is rounded
+// to the pool's type for the second product (by 2^-9 or 2^-12 of a weight at most
+// and averaged over the keys: at the level of the output's own rounding); the
+// sum l is of the unrounded weights.
+template <typename T, int D, int NST>
+__device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, const Totals& tot, uint32_t ring,
+                                          int64_t worker) {
+  constexpr int CH = D / 8;  // 16-byte chunks per row
+  constexpr uint32_t STAGE = stage_bytes(D), NONE = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  // rows of a tile sit `D * 2` bytes apart with their 16-byte chunks permuted
+  // by the row, so the eight rows of a matrix load fall on different banks
+  auto chunk_at = [](int row, int c) -> uint32_t {
+    return (uint32_t)(row * (D * 2) + ((c ^ (CH >= 8 ? (row & 7) : ((row >> 1) & 3))) << 4));
+  };
+
+  // ---- the copies' side: what goes into the next stage
+  Run ahead(p, plan, tot, worker, lane);
+  Run run = ahead;
+  Item ld;
+  int32_t ld_j = 0, ld_n = 0;   // stage of item ld (0: Q), its stages
+  uint32_t row = NONE;          // the coming stage: the row of this lane (of D elements; lanes 0-15)
+  int kind = 0;                 // and what it is: 0 nothing, 1 Q, 2 a tile
+  auto plan_stage = [&] {
+    if (ld_j == ld_n) {
+      kind = 0;
+      if (!ahead.next(p, ld)) return;
+      ld_j = 0;
+      ld_n = 1 + cdiv(ld.t1 - ld.t0, KT);
+    }
+    row = NONE;
+    if (ld_j == 0) {
+      kind = 1;
+      const int32_t r = ld.r0 + lane;
+      if (lane < ld.nrows) row = (uint32_t)((ld.b0 + r / p.G) * (int32_t)p.H + ld.kvh * p.G + r % p.G);
+    } else {
+      kind = 2;
+      const int32_t t = ld.t0 + (ld_j - 1) * KT + lane;
+      if (lane < KT && t < ld.t1) {
+        const int32_t page = p.bs_shift >= 0 ? t >> p.bs_shift : t / (int32_t)p.BS;
+        int32_t blk = __ldg(p.block_tables + (int64_t)ld.table * p.MB + page);
+        if (blk < 0 || blk >= p.NB) {
+          report(p.dev_status, PA_DEVERR_BLOCK_ID);
+          blk = 0;
+        }
+        row = (uint32_t)(((int64_t)blk * p.BS + (t - page * (int32_t)p.BS)) * p.HKV + ld.kvh);
+      }
+    }
+    ++ld_j;
+  };
+  // Rows of no key or query are zeros: their scores are masked, and no weight
+  // of zero meets a NaN of an unwritten row.
+  auto fill = [&](uint32_t st, int kind, uint32_t row) {
+    if (kind) {
+      const char* a = static_cast<const char*>(kind == 1 ? p.q : p.k);
+#pragma unroll
+      for (int i = 0; i < KT * CH / 32; ++i) {
+        const int idx = i * 32 + lane, r = idx / CH, c = idx % CH;
+        const uint32_t pr = __shfl_sync(0xffffffffu, row, r);
+        const int bytes = pr == NONE ? 0 : 16;
+        const int64_t off = bytes ? ((int64_t)pr * CH + c) * 16 : 0;
+        cp_async16(ring + st + chunk_at(r, c), a + off, bytes);
+        if (kind == 2)
+          cp_async16(ring + st + KT * D * 2 + chunk_at(r, c), static_cast<const char*>(p.v) + off, bytes);
+      }
+    }
+    cp_async_commit();
+  };
+  uint32_t st_ld = 0, st = 0;  // stage to fill, stage to read
+  auto step = [](uint32_t& s) { s = s + STAGE == NST * STAGE ? 0 : s + STAGE; };
+  plan_stage();
+#pragma unroll 1
+  for (int i = 0; i < NST - 1; ++i) {
+    const uint32_t r = row;
+    const int k = kind;
+    plan_stage();
+    fill(st_ld, k, r);
+    step(st_ld);
+  }
+  // The stage at `st` is there, and the one before it, which every lane has
+  // left, is being filled.
+  auto arrive = [&] {
+    const uint32_t r = row;
+    const int k = kind;
+    plan_stage();
+    cp_async_wait<NST - 2>();
+    __syncwarp();
+    fill(st_ld, k, r);
+    step(st_ld);
+  };
+
+  // ---- the products' side
+  const int mi = lane >> 3, mr = lane & 7;  // matrix and row that this lane addresses
+  Item im;
+  while (run.next(p, im)) {
+    arrive();
+    uint32_t qa[D / 16][4];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) ldsm4(qa[kk], ring + st + chunk_at(mr + 8 * (mi & 1), 2 * kk + (mi >> 1)));
+    step(st);
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int valid = im.t1 - im.t0; valid > 0; valid -= KT) {
+      arrive();
+      const uint32_t ks = ring + st, vs = ks + KT * D * 2;
+      float s[2][4] = {};
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];
+        ldsm4(b, ks + chunk_at(mr + 8 * (mi >> 1), 2 * kk + (mi & 1)));
+        mma(s[0], qa[kk], b[0], b[1], (T*)nullptr);
+        mma(s[1], qa[kk], b[2], b[3], (T*)nullptr);
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = 8 * n + 2 * (lane & 3) + (e & 1) < valid;
+          s[n][e] = in ? s[n][e] * p.qscale : -INFINITY;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+        }
+      float alpha[2], base[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+        const float mn = fmaxf(m[hf], mx[hf]);
+        base[hf] = mn == -INFINITY ? 0.f : mn;  // only -inf scores so far
+        alpha[hf] = fast_exp2(m[hf] - base[hf]);
+        m[hf] = mn;
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= alpha[0];
+          o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1];
+          o[i][3] *= alpha[1];
+        }
+        l[0] *= alpha[0];
+        l[1] *= alpha[1];
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = fast_exp2(s[n][e] - base[e >> 1]);
+          l[e >> 1] += s[n][e];
+        }
+      const uint32_t pa[4] = {pack2(s[0][0], s[0][1], (T*)nullptr), pack2(s[0][2], s[0][3], (T*)nullptr),
+                              pack2(s[1][0], s[1][1], (T*)nullptr), pack2(s[1][2], s[1][3], (T*)nullptr)};
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd) {
+        uint32_t b[4];
+        ldsm4t(b, vs + chunk_at(mr + 8 * (mi & 1), 2 * dd + (mi >> 1)));
+        mma(o[2 * dd], pa, b[0], b[1], (T*)nullptr);
+        mma(o[2 * dd + 1], pa, b[2], b[3], (T*)nullptr);
+      }
+      step(st);
+    }
+
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+      const int r = (lane >> 2) + 8 * hf;
+      if (r < im.nrows) {
+        const int64_t out = im.prow + r;
+        if ((lane & 3) == 0) p.part_ml[out] = make_float2(m[hf], l[hf]);
+        float* dst = p.part_o + out * D + 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+// `after`: as a programmatic dependent of the launch before it.
 template <typename K, typename A>
-inline cudaError_t launch_pdl(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const A& p) {
+inline cudaError_t launch(K kern, int64_t grid, int block, size_t smem, cudaStream_t s, const A& p, bool after) {
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// One tensor-memory launch on the plan in p (shared_tc.cu).
+// The attention launch with the tensor-memory part (shared_tc.cu): which pools
+// it can load, how many of a CTA's warps take 16-key tiles, the launch.
 bool tc_takes(int64_t D, int64_t BS, int64_t NB);
+constexpr int kTcWarps = 8;
 int launch_tc(const Params& p, int dtype, int64_t D, cudaStream_t s);
 
 }  // namespace shared

@@ -1,11 +1,14 @@
-// shared_tc.cu -- prefixes shared by many query rows, on the sm_100a tensor
-// cores: the members' query heads of one KV head are the rows of S = Q K^T and
-// O = P V with S, P and O in tensor memory.
+// shared_tc.cu -- the attention launch of the shared-prefix decode for pools
+// that tiled TMA can load (whole 16-row groups inside a page, head_dim 64 or
+// 128): first the prefixes shared by many query rows, on the sm_100a tensor
+// cores with S, P and O in tensor memory, then the rest, a warp at a time
+// (shared.cuh).
 //
-// A CTA (one per SM) takes its run of 128-key tiles (shared.cuh) and walks the
-// units that it crosses.  Two softmax warpgroups run two chains: rows 0-127 and
-// 128-255 of a unit, or, in a unit of at most 128 rows, the same rows on every
-// other tile, so that one chain's exponentials overlap the other's products.
+// A CTA (one per SM) takes its run of 128-key tiles and walks the units that it
+// crosses: the members' query heads of one KV head are the rows of S = Q K^T and
+// O = P V.  Two softmax warpgroups run two chains: rows 0-127 and 128-255 of a
+// unit, or, in a unit of at most 128 rows, the same rows on every other tile,
+// so that one chain's exponentials overlap the other's products.
 // Thread = row = TMEM lane: it reads its 128 scores, keeps the row's reference
 // maximum and sum in fp32 and writes P over S.  Two warps feed K and V by tiled
 // TMA, 16 rows at a time through the pages; one thread issues the MMAs.
@@ -24,7 +27,6 @@
 namespace pa {
 namespace shared {
 
-using prefill::pack2;
 using prefill::sw128_offset;
 using prefill::v_group_sanitised;
 using prefill::warp_wait;
@@ -40,10 +42,14 @@ static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kTcThreads * 168, "regist
 template <int D> struct TcCfg {
   static constexpr int NH = D / 64;                    // 128-byte column halves of a row
   static constexpr uint32_t TILE = 128 * D * 2;        // Q of a chain, K or V of a tile
-  static constexpr int NK = D == 128 ? 3 : 4, NV = D == 128 ? 2 : 4;
+  static constexpr int NK = D == 128 ? 3 : 6, NV = D == 128 ? 2 : 6;
   static constexpr uint32_t OFF_K = 2 * TILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;
   static constexpr uint32_t N_BARS = 2 * NK + 2 * NV + 2 * 4;
   static constexpr uint32_t SMEM = OFF_BAR + N_BARS * 8 + 16 + 1024;  // + alignment slack
+  // afterwards the warps' rings, in the same bytes
+  static constexpr int STAGES = (int)(OFF_BAR / kTcWarps / stage_bytes(D));
+  static constexpr uint32_t RING = STAGES * stage_bytes(D);
+  static_assert(plan_scratch(kPlanMax, kPlanMax) <= OFF_BAR, "the plan's scratch comes before all");
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
   // tensor memory columns: S (and P) of the chains, O of the chains
   static constexpr uint32_t COL_S = 0, COL_O = 256;
@@ -65,18 +71,20 @@ struct TcItem {
 struct Walk {
   int64_t x, end;
   int32_t at;
-  __device__ __forceinline__ Walk(const Params& p, const Totals& tot, int64_t worker, int lane) {
+  const Group* groups;
+  __device__ __forceinline__ Walk(const Params& p, const Plan& plan, const Totals& tot, int64_t worker, int lane) {
+    groups = plan.groups;
     x = end = 0;
     at = 0;
     if (worker < tot.tc_workers) {
       x = first_tile(worker, tot.tc_tiles, tot.tc_workers);
       end = first_tile(worker + 1, tot.tc_tiles, tot.tc_workers);
     }
-    if (x < end) at = find<1>(p.groups, (int32_t)p.NG, x, lane);
+    if (x < end) at = find<1>(groups, (int32_t)p.NG, x, lane);
   }
   __device__ __forceinline__ bool next(const Params& p, int64_t worker, TcItem& im) {
     while (x < end) {
-      const Group gp = load_plan(p.groups + at);
+      const Group gp = load_plan(groups + at);
       const int32_t rows = gp.n * p.G, ry = cdiv(rows, TC_ROWS), nt = cdiv(gp.prefix, TC_KT);
       const int64_t done = x - gp.tile0[1];
       if (!gp.tc || done >= (int64_t)p.HKV * ry * nt) {
@@ -120,6 +128,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   int32_t* abort_s = reinterpret_cast<int32_t*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  pdl_trigger();
+  const Plan plan = take_plan(p, smem);
+  // the scratch in shared memory, written and read as usual, is the TMA's next
+  tc::fence_proxy_async_smem();
   if (threadIdx.x == 0) {
     for (int s = 0; s < NK; ++s) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
     for (int s = 0; s < NV; ++s) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
@@ -140,11 +152,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-  pdl_trigger();
-  const Totals tot = load_plan(p.totals);
+  const Totals tot = load_plan(plan.totals);
   const int64_t worker = blockIdx.x;
-  Walk walk(p, tot, worker, lane);
+  Walk walk(p, plan, tot, worker, lane);
   TcItem im;
 
   if (warp < 8) {
@@ -270,6 +280,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       }
     }
     if (!ok && lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
+    // Both chains done: every product has been taken, and the shared memory is
+    // free for the rings of the warps' own work
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
+      warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, (int64_t)warp * gridDim.x + blockIdx.x);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kMmaWarp) {
@@ -381,7 +396,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           if (lane < NBOX && !manual) tc::tma_load_3d(dst, map, hf * 64, im.kvh, row, &full[st]);
         }
       }
-      if (!ok && lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
+      if (!ok) {
+        if (lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
+        // copies still in flight land before the CTA gives up its memory
+        for (uint32_t i = n > (uint32_t)n_st ? n - n_st : 0; i < n; ++i)
+          (void)mbar_wait(&full[i % n_st], (i / n_st) & 1);
+      }
     }
   }
 
@@ -396,7 +416,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
 // True when the tensor-memory kernel can load these pools: whole 16-row groups
 // inside a page, row coordinates in 32 bits.
 bool tc_takes(int64_t D, int64_t BS, int64_t NB) {
-  return (D == 64 || D == 128) && BS % 16 == 0 && NB * BS <= 0x7fffffff;
+  return (D == 64 || D == 128) && BS % 16 == 0 && NB > 0 && NB * BS <= 0x7fffffff;
 }
 
 template <typename T, int D>
@@ -416,7 +436,7 @@ static int launch_tc_typed(const TcParams& tp, cudaStream_t s) {
       done.push_back(dev);
     }
   }
-  return cuda_status(launch_pdl(kern, dim3((unsigned)tp.p.tc_ctas), dim3(kTcThreads), C::SMEM, s, tp));
+  return cuda_status(launch(kern, tp.p.tc_ctas, kTcThreads, C::SMEM, s, tp, tp.p.planned));
 }
 
 int launch_tc(const Params& p, int dtype, int64_t D, cudaStream_t s) {

@@ -320,3 +320,27 @@ def test_workspace_and_alignment_refusals():
     assert call(wn=n.value - 1) == _lib.PA_ERR_WORKSPACE and call(w=None) == _lib.PA_ERR_WORKSPACE
     assert call(qp=ptr(q) + 2) == _lib.PA_ERR_ALIGNMENT and call(w=ptr(ws) + 4) == _lib.PA_ERR_ALIGNMENT
     assert call(nb=1 << 27) == _lib.PA_ERR_TOO_LARGE
+
+
+@pytest.mark.parametrize("D,BS", [(64, 16), (32, 16), (128, 4)])
+def test_many_sequences_and_many_groups(D, BS):
+    """More sequences, then more groups, than every CTA plans for by itself."""
+    rng = np.random.default_rng(D)
+    ctx = (50 + rng.integers(0, 30, 1100)).tolist()
+    ctx[7] = ctx[500] = ctx[1099] = 0
+    run_and_check(make(16, 4, 2, D, torch.bfloat16, BS, [3, 500, 501, 1100], [50, 20, 33], ctx), torch.bfloat16)
+    starts = list(range(0, 2402, 2))
+    ctx = (20 + rng.integers(0, 20, 2403)).tolist()
+    run_and_check(make(17, 2, 2, D, torch.float16, BS, starts, rng.integers(0, 21, len(starts) - 1).tolist(), ctx),
+                  torch.float16)
+
+
+@pytest.mark.parametrize("members", [9, 32, 33, 65, 100])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_groups_in_tensor_memory(members, dtype, D):
+    """Prefixes long enough for the tensor cores: units of at most 128 rows and more, last units of few rows, a
+    last tile of one key, groups that the warps take beside them."""
+    ctx = tails(8192 + 1, [b % 40 for b in range(members)]) + tails(31, [4, 9]) + tails(5000, [b for b in range(members)])
+    starts = [0, members, members + 2, 2 * members + 2]
+    run_and_check(make(members, 16, 4, D, dtype, 16, starts, [8193, 31, 5000], ctx), dtype)
+    run_and_check(make(members, 16, 4, D, dtype, 32, starts, [8193, 31, 5000], ctx), dtype, scale=-0.1)
