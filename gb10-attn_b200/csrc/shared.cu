@@ -26,7 +26,7 @@ namespace shared {
 // The plan as a launch of its own, for more sequences or groups than kPlanMax.
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
-  make_plan(p, plan_at(p, 0), reinterpret_cast<int32_t*>(p.plan + p.scratch_off), true);
+  make_plan(p, plan_at(p, 0), p.plan + p.scratch_off, true);
 }
 
 // All of the work by warps: pools that the tensor-memory part does not load.
@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   if (sp.group >= 0 && sp.from > 0) {
     const Group gp = load_plan(plan.groups + sp.group);
     const int32_t rows = gp.n * p.G, r = ((int32_t)b - gp.b0) * p.G + g;
-    const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R), nt = cdiv(gp.prefix, gp.tc ? TC_KT : KT);
+    const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R);
+    const int32_t nt = gp.tc ? tc_unit_tiles(gp.prefix) : unit_tiles(gp.prefix);
     const int64_t tiles = gp.tc ? tot.tc_tiles : tot.tiles, workers = gp.tc ? tot.tc_workers : tot.workers;
     const int32_t u = kv * ry + r / R;
     const int64_t a = (gp.tc ? gp.tile0[1] : gp.tile0[0]) + (int64_t)u * nt;
@@ -85,8 +86,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
     if (gp.tc && rows - r / R * R <= R / 2) pre_step = R / 2, n_pre *= 2;
   }
   if (sp.ctx > sp.from) {
-    const int32_t nt = cdiv(sp.ctx - sp.from, KT), u = kv * own_y + g / ROWS;
-    const int64_t a = sp.tile0[0] + (int64_t)u * nt;
+    const int32_t nt = unit_tiles(sp.ctx - sp.from), u = kv * own_y + g / ROWS;
+    const int64_t a = tot.prefix_tiles + sp.tile0[0] + (int64_t)u * nt;
     const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
     n_own = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
     own0 = p.own_row0 + (b * p.HKV * own_y + u + w0) * own_rows + g % ROWS;
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   for (int c0 = 0; c0 < n; c0 += 32) {
     float2 ml = make_float2(-INFINITY, 0.f);
     if (c0 + lane < n) ml = p.part_ml[piece(c0 + lane)];
-    const bool none = ml.x == -INFINITY && ml.y == 0.f;  // without keys, or only scores of -inf: O not read
+    const bool none = ml.x == -INFINITY && ml.y == 0.f;  // without keys, or only scores of -inf: O not used
     float top = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -122,22 +123,20 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
       const float* src = p.part_o + piece(c0 + c) * D + lane * V;
       float x[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = 0.f;
-      if (read >> c & 1)
-#pragma unroll
-        for (int i = 0; i < E / V; ++i) {
-          if constexpr (V == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
-            x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
-          } else if constexpr (V == 2) {
-            const float2 f = *reinterpret_cast<const float2*>(src);
-            x[0] = f.x, x[1] = f.y;
-          } else {
-            x[0] = *src;
-          }
+      for (int i = 0; i < E / V; ++i) {
+        if constexpr (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
+          x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
+        } else if constexpr (V == 2) {
+          const float2 f = *reinterpret_cast<const float2*>(src);
+          x[0] = f.x, x[1] = f.y;
+        } else {
+          x[0] = *src;
         }
+      }
+      const bool in = read >> c & 1;  // (loaded in any case, so that the loads need not wait for ml)
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(wc, x[e], acc[e]);
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(wc, in ? x[e] : 0.f, acc[e]);
     }
   }
   // no key, or only scores of -inf: L = 0, so out is NaN and lse -inf

@@ -25,6 +25,9 @@ constexpr int TC_ROWS = 256;
 // [w T / W, (w + 1) T / W), so a unit is cut where a worker's run ends.  A piece
 // is the overlap of unit u and worker w; u + w grows strictly from piece to
 // piece, so it numbers the pieces' slots for partials, with no table of them.
+//   A unit counts as a few tiles more than it has, before its first: what taking
+// it up costs (its queries, the partials of the one before), so that workers
+// that meet a unit's start have less to read.  A piece of these alone is empty.
 //   The prefixes of groups with many rows are done in tensor memory
 // (shared_tc.cu), with tiles, units and workers (CTAs) of their own, numbered
 // the same way.
@@ -34,7 +37,7 @@ struct alignas(16) Group {
   int32_t unit0[2], tc, pad;    // first unit; whether it is done in tensor memory
 };
 struct alignas(16) Seq {
-  long long tile0[1];
+  long long tile0[1];             // counted from the end of the prefixes
   int32_t from, ctx, group, pad;  // own tokens from .. ctx - 1; its group or -1
 };
 struct alignas(16) Totals {
@@ -117,30 +120,42 @@ __device__ __forceinline__ Plan plan_at(const Params& p, int64_t copy) {
 // Sequences and groups up to which every CTA makes the plan itself, in shared
 // memory: one launch less, which small calls notice.
 constexpr int kPlanMax = 1024;
-__host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) { return (2 * B + 3 * (NG + 1)) * 4; }
+constexpr int64_t kScanBytes = 2 * 32 * 32 + 16;  // the scans' sums, a counter
+__host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
+  return kScanBytes + (2 * B + 3 * (NG + 1)) * 4;
+}
 
-constexpr int kMinTiles = 2;    // 16-key tiles per warp when there are few
+constexpr int kMinTiles = 4;    // 16-key tiles per warp when there are few
 constexpr int kTcMinTiles = 3;  // 128-key tiles per CTA below which the warps do all
+#ifndef KUC
+#define KUC 2
+#define KTUC 3
+#endif
+constexpr int kUnitCost = KUC;     // tiles that a unit costs beside its own
+constexpr int kTcUnitCost = KTUC;
 
-// Exclusive scan of N values over the block on top of the running totals `base`.
+// Tiles that a unit of `keys` keys counts as.
+__host__ __device__ __forceinline__ int32_t unit_tiles(int32_t keys) { return keys ? cdiv(keys, KT) + kUnitCost : 0; }
+__host__ __device__ __forceinline__ int32_t tc_unit_tiles(int32_t keys) {
+  return keys ? cdiv(keys, TC_KT) + kTcUnitCost : 0;
+}
+
+// Exclusive scan of N values over the block on top of the running totals
+// `base`; warp_sums: one entry a warp, not in use by an earlier scan any more.
 template <int N> struct Sums {
   long long v[N];
 };
 template <int N>
 __device__ __forceinline__ Sums<N> block_scan(const Sums<N>& x, Sums<N>* warp_sums, Sums<N>& base) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  auto warp_scan = [&](Sums<N> s) {
+  Sums<N> s = x;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
+  for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const long long y = __shfl_up_sync(0xffffffffu, s.v[i], o);
-        if (lane >= o) s.v[i] += y;
-      }
-    return s;
-  };
-  const Sums<N> s = warp_scan(x);
-  __syncthreads();
+    for (int i = 0; i < N; ++i) {
+      const long long y = __shfl_up_sync(0xffffffffu, s.v[i], o);
+      if (lane >= o) s.v[i] += y;
+    }
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
   Sums<N> r = {}, all = {};
@@ -160,13 +175,13 @@ __device__ __forceinline__ Sums<N> block_scan(const Sums<N>& x, Sums<N>* warp_su
 
 // One CTA makes the plan; `scratch`: plan_scratch() bytes, in shared memory or
 // its own part of the workspace.  Ends with a barrier.
-__device__ __forceinline__ void make_plan(const Params& p, const Plan& out, int32_t* scratch, bool tell) {
-  __shared__ Sums<3> sums[32];
-  __shared__ unsigned long long tc_work;
+__device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void* scratch, bool tell) {
+  auto sums = static_cast<Sums<4>(*)[32]>(scratch);
+  unsigned long long& tc_work = *reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + 2 * 32 * 32);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
   const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
-  int32_t *ctx = scratch, *grp = ctx + B, *gs = grp + B, *pre = gs + NG + 1, *lead = pre + NG + 1;
+  int32_t *ctx = reinterpret_cast<int32_t*>(static_cast<char*>(scratch) + kScanBytes), *grp = ctx + B, *gs = grp + B, *pre = gs + NG + 1, *lead = pre + NG + 1;
   if (tid == 0) tc_work = 0;
   int far = 0;
   for (int32_t b = tid; b < B; b += threads) {
@@ -203,45 +218,42 @@ __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, int3
       pre[g] = prefix;
       lead[g] = first;
       if (p.tc_rows && (e - a) * G >= p.tc_rows)
-        atomicAdd(&tc_work, (unsigned long long)HKV * cdiv((e - a) * G, TC_ROWS) * cdiv(prefix, TC_KT));
+        atomicAdd(&tc_work, (unsigned long long)HKV * cdiv((e - a) * G, TC_ROWS) * tc_unit_tiles(prefix));
     }
   }
   __syncthreads();
   const bool use_tc = p.tc_rows && tc_work >= (unsigned long long)kTcMinTiles * p.tc_ctas;
-  Sums<3> base = {};  // tiles of the warps and of the tensor memory, units (tensor memory's in the high half)
-  for (int32_t g0 = 0; g0 < groups; g0 += threads) {
-    const int32_t g = g0 + tid;
-    Sums<3> x = {};
-    int32_t n = 0, prefix = 0, tc = 0;
-    if (g < groups) {
-      n = gs[g + 1] - gs[g];
-      prefix = pre[g];
+  // running counts: of the groups' tiles (the warps', the tensor memory's) and
+  // units (the tensor memory's in the high half), and of the sequences' tiles
+  Sums<4> base = {};
+  for (int32_t i0 = 0, k = 0; i0 < max(B, groups); i0 += threads, k ^= 1) {
+    const int32_t i = i0 + tid;
+    Sums<4> x = {};
+    int32_t n = 0, prefix = 0, tc = 0, from = 0, g = -1;
+    if (i < groups) {
+      n = gs[i + 1] - gs[i];
+      prefix = pre[i];
       tc = use_tc && n * G >= p.tc_rows;
       const long long units = (long long)HKV * cdiv(n * G, tc ? TC_ROWS : ROWS);
-      x = tc ? Sums<3>{{0, units * cdiv(prefix, TC_KT), units << 32}} : Sums<3>{{units * cdiv(prefix, KT), 0, units}};
+      x = tc ? Sums<4>{{0, units * tc_unit_tiles(prefix), units << 32, 0}}
+             : Sums<4>{{units * unit_tiles(prefix), 0, units, 0}};
     }
-    const Sums<3> at = block_scan(x, sums, base);
-    if (g < groups)
-      out.groups[g] = Group{{at.v[0], at.v[1]}, gs[g], n, lead[g], prefix,
+    if (i < B) {
+      g = grp[i];
+      if (g >= 0) from = min(pre[g], ctx[i]);
+      x.v[3] = (long long)HKV * cdiv(G, ROWS) * unit_tiles(ctx[i] - from);
+    }
+    const Sums<4> at = block_scan(x, sums[k], base);
+    if (i < groups)
+      out.groups[i] = Group{{at.v[0], at.v[1]}, gs[i], n, lead[i], prefix,
                             {(int32_t)(at.v[2] & 0xffffffff), (int32_t)(at.v[2] >> 32)}, tc, 0};
+    if (i < B) out.seqs[i] = Seq{{at.v[3]}, from, ctx[i], g, 0};
   }
-  Sums<1> own = {{base.v[0]}};
-  for (int32_t b0 = 0; b0 < B; b0 += threads) {
-    const int32_t b = b0 + tid;
-    Sums<1> x = {};
-    int32_t from = 0, g = -1;
-    if (b < B) {
-      g = grp[b];
-      if (g >= 0) from = min(pre[g], ctx[b]);
-      x.v[0] = (long long)HKV * cdiv(G, ROWS) * cdiv(ctx[b] - from, KT);
-    }
-    const Sums<1> at = block_scan(x, reinterpret_cast<Sums<1>*>(sums), own);
-    if (b < B) out.seqs[b] = Seq{{at.v[0]}, from, ctx[b], g, 0};
+  if (tid == 0) {
+    const int64_t tiles = base.v[0] + base.v[3], tc_tiles = base.v[1];
+    *out.totals = Totals{base.v[0], tiles, min((int64_t)p.warps, max((tiles + kMinTiles - 1) / kMinTiles, (int64_t)1)),
+                         tc_tiles, min((int64_t)p.tc_ctas, max(tc_tiles, (int64_t)1))};
   }
-  if (tid == 0)
-    *out.totals = Totals{base.v[0], own.v[0],
-                         min((int64_t)p.warps, max(((int64_t)own.v[0] + kMinTiles - 1) / kMinTiles, (int64_t)1)),
-                         base.v[1], min((int64_t)p.tc_ctas, max((int64_t)base.v[1], (int64_t)1))};
   __syncthreads();
 }
 
@@ -252,7 +264,7 @@ __device__ __forceinline__ Plan take_plan(const Params& p, void* smem_scratch) {
     return plan_at(p, 0);
   }
   const Plan plan = plan_at(p, blockIdx.x);
-  make_plan(p, plan, static_cast<int32_t*>(smem_scratch), blockIdx.x == 0);
+  make_plan(p, plan, smem_scratch, blockIdx.x == 0);
   return plan;
 }
 
@@ -282,10 +294,11 @@ struct Run {
     at = u = j = units = 0;
     pre = false;
     if (w >= tot.workers) return;
-    const int64_t x = first_tile(w, tot.tiles, tot.workers);
+    int64_t x = first_tile(w, tot.tiles, tot.workers);
     left = first_tile(w + 1, tot.tiles, tot.workers) - x;
     if (left == 0) return;
     pre = x < tot.prefix_tiles;
+    if (!pre) x -= tot.prefix_tiles;
     at = pre ? find<0>(groups, (int32_t)p.NG, x, lane) : find<0>(seqs, (int32_t)p.B, x, lane);
     const int64_t done = x - entry(p);
     u = (int32_t)(done / nt);
@@ -312,7 +325,7 @@ struct Run {
       to = sp.ctx;
       slot = p.own_row0 + (int64_t)at * p.HKV * cdiv(p.G, ROWS) * min(p.G, ROWS);
     }
-    nt = cdiv(to - from, KT);
+    nt = unit_tiles(to - from);
     unit_y = cdiv(rows, ROWS);
     units = nt ? (int32_t)p.HKV * unit_y : 0;
     return tile0;
@@ -330,8 +343,8 @@ struct Run {
     im.kvh = u / unit_y;
     im.r0 = (u - im.kvh * unit_y) * ROWS;
     im.nrows = min(ROWS, rows - im.r0);
-    im.t0 = from + j * KT;
-    im.t1 = min(to, im.t0 + n * KT);
+    im.t0 = from + max(j - kUnitCost, 0) * KT;
+    im.t1 = min(to, from + max(j + n - kUnitCost, 0) * KT);
     im.prow = slot + (u + worker) * (pre ? ROWS : min(p.G, ROWS));
     left -= n;
     j += n;
@@ -407,10 +420,16 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
   // ---- the copies' side: what goes into the next stage
   Run ahead(p, plan, tot, worker, lane);
   Run run = ahead;
-  Item ld;
+  Item ld = {};
   int32_t ld_j = 0, ld_n = 0;   // stage of item ld (0: Q), its stages
   uint32_t row = NONE;          // the coming stage: the row of this lane (of D elements; lanes 0-15)
   int kind = 0;                 // and what it is: 0 nothing, 1 Q, 2 a tile
+  int32_t ids = 0, page0 = 0;   // block ids of pages page0 + lane of item ld
+  auto page_of = [&](int32_t t) { return p.bs_shift >= 0 ? t >> p.bs_shift : t / (int32_t)p.BS; };
+  auto load_ids = [&](int32_t t) {
+    page0 = page_of(t);
+    ids = page0 + lane <= page_of(ld.t1 - 1) ? __ldg(p.block_tables + (int64_t)ld.table * p.MB + page0 + lane) : 0;
+  };
   auto plan_stage = [&] {
     if (ld_j == ld_n) {
       kind = 0;
@@ -421,14 +440,15 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
     row = NONE;
     if (ld_j == 0) {
       kind = 1;
+      if (ld_n > 1) load_ids(ld.t0);  // needed a stage later
       const int32_t r = ld.r0 + lane;
       if (lane < ld.nrows) row = (uint32_t)((ld.b0 + r / p.G) * (int32_t)p.H + ld.kvh * p.G + r % p.G);
     } else {
       kind = 2;
-      const int32_t t = ld.t0 + (ld_j - 1) * KT + lane;
+      const int32_t t0 = ld.t0 + (ld_j - 1) * KT, t = t0 + lane, page = page_of(t);
+      if (page_of(min(t0 + KT, ld.t1) - 1) >= page0 + 32) load_ids(t0);
+      int32_t blk = __shfl_sync(0xffffffffu, ids, page - page0);
       if (lane < KT && t < ld.t1) {
-        const int32_t page = p.bs_shift >= 0 ? t >> p.bs_shift : t / (int32_t)p.BS;
-        int32_t blk = __ldg(p.block_tables + (int64_t)ld.table * p.MB + page);
         if (blk < 0 || blk >= p.NB) {
           report(p.dev_status, PA_DEVERR_BLOCK_ID);
           blk = 0;

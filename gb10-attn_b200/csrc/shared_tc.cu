@@ -61,7 +61,7 @@ struct TcParams {
 };
 
 // A unit's part of a CTA's run: rows r0 .. r0 + rows - 1 of the group (at most
-// 256), KV head kvh, tiles j0 .. j0 + n - 1, keys below `prefix`.
+// 256), KV head kvh, tiles j0 .. j0 + n - 1 (n may be 0), keys below `prefix`.
 struct TcItem {
   int32_t table, b0, r0, rows, kvh, j0, n, prefix;
   int64_t prow;  // first partial row
@@ -85,15 +85,16 @@ struct Walk {
   __device__ __forceinline__ bool next(const Params& p, int64_t worker, TcItem& im) {
     while (x < end) {
       const Group gp = load_plan(groups + at);
-      const int32_t rows = gp.n * p.G, ry = cdiv(rows, TC_ROWS), nt = cdiv(gp.prefix, TC_KT);
+      const int32_t rows = gp.n * p.G, ry = cdiv(rows, TC_ROWS), nt = tc_unit_tiles(gp.prefix);
       const int64_t done = x - gp.tile0[1];
       if (!gp.tc || done >= (int64_t)p.HKV * ry * nt) {
         ++at;
         continue;
       }
       const int32_t u = (int32_t)(done / nt);
-      im.j0 = (int32_t)(done - (int64_t)u * nt);
-      im.n = (int32_t)min((int64_t)(nt - im.j0), end - x);
+      const int32_t j = (int32_t)(done - (int64_t)u * nt), n = (int32_t)min((int64_t)(nt - j), end - x);
+      im.j0 = max(j - kTcUnitCost, 0);
+      im.n = max(j + n - kTcUnitCost, 0) - im.j0;
       im.table = gp.table;
       im.b0 = gp.b0;
       im.kvh = u / ry;
@@ -101,7 +102,7 @@ struct Walk {
       im.rows = min(TC_ROWS, rows - im.r0);
       im.prefix = gp.prefix;
       im.prow = p.tc_row0 + (gp.unit0[1] + u + worker) * TC_ROWS;
-      x += im.n;
+      x += n;
       return true;
     }
     return false;
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       const bool by_keys = im.rows <= 128;
       const int row = by_keys ? r : 128 * c + r;  // of the unit
       const int tiles = by_keys ? (im.n - c + 1) / 2 : im.n;
-      {
+      if (im.n > 0) {
         unsigned char* qd = smem + c * C::TILE;
         const int rr = im.r0 + row;
         const bool in = row < im.rows;
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       uint32_t uses0 = 0, uses1 = 0;    // tiles of the chains so far
       bool ok = true;
       while (walk.next(p, worker, im)) {
-        if (lane != 0 || !ok) continue;  // (the other lanes only walk along)
+        if (lane != 0 || !ok || im.n == 0) continue;  // (the other lanes only walk along)
         const bool by_keys = im.rows <= 128;
         // element e: chain e & 1 on tile e (by keys) or e / 2
         const int E = by_keys ? im.n : 2 * im.n;
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       uint32_t n = 0;
       bool ok = true;
       while (ok && walk.next(p, worker, im)) {
+        if (im.n == 0) continue;
         const int32_t* table = p.block_tables + (int64_t)im.table * p.MB;
         auto row_of = [&](int j) -> int32_t {  // pool row of this lane's group of tile j
           const int32_t t = j * TC_KT + g16 * 16;
