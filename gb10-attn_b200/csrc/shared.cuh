@@ -14,7 +14,7 @@ constexpr int ROWS = 16;  // query rows per item (the M of one mma)
 
 // tensor-memory part: keys per tile, rows per unit (two chains of 128; a unit
 // of at most 128 rows gives both chains the same rows and every other tile)
-constexpr int TC_KT = 128;
+constexpr int TC_KT = 64;
 constexpr int TC_ROWS = 256;
 
 // The work, counted in tiles of KT keys: first the groups' prefixes, then the
@@ -126,10 +126,12 @@ __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
 }
 
 constexpr int kMinTiles = 4;    // 16-key tiles per warp when there are few
-constexpr int kTcMinTiles = 3;  // 128-key tiles per CTA below which the warps do all
+constexpr int kTcMinTiles = 6;  // 64-key tiles per CTA below which the warps do all
 #ifndef KUC
 #define KUC 2
-#define KTUC 3
+#endif
+#ifndef KTUC
+#define KTUC 5
 #endif
 constexpr int kUnitCost = KUC;     // tiles that a unit costs beside its own
 constexpr int kTcUnitCost = KTUC;

@@ -9,9 +9,9 @@
 // O = P V.  Two softmax warpgroups run two chains: rows 0-127 and 128-255 of a
 // unit, or, in a unit of at most 128 rows, the same rows on every other tile,
 // so that one chain's exponentials overlap the other's products.
-// Thread = row = TMEM lane: it reads its 128 scores, keeps the row's reference
-// maximum and sum in fp32 and writes P over S.  Two warps feed K and V by tiled
-// TMA, 16 rows at a time through the pages; one thread issues the MMAs.
+// Thread = row = TMEM lane: it reads its 64 scores of a tile, keeps the
+// row's reference maximum and sum in fp32 and writes P over S.  Two warps feed K and V by tiled
+// TMA, 16 rows at a time through the pages; one thread per chain issues its MMAs.
 //   Precision: one 16-bit product each for S (Q and K as they are, products
 // exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be; the
 // sum l is of the unrounded weights).  The scale is applied to S in fp32.
@@ -32,28 +32,51 @@ using prefill::v_group_sanitised;
 using prefill::warp_wait;
 using prefill::warp_wait_rx;
 
-constexpr int kMmaWarp = 8, kKWarp = 9, kVWarp = 10;
+constexpr int kMmaWarp = 8, kKWarp = 10, kVWarp = 11;  // (an issuer per chain: 8 and 9)
 constexpr int kTcThreads = 384;
-// 384 threads launched at 168 registers (64512): the softmax warpgroups take
-// 224, the rest keep 56: 256 x 224 + 128 x 56 = 64512.
-constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kTcThreads * 168, "register split");
+// 384 threads launched at 168 registers (64512).  After the tensor-memory part
+// the issuing and loading warps give theirs up and the warps' own work takes
+// 240: 256 x 240 + 128 x 24 = 64512.
+constexpr int kWorkRegs = 240, kDoneRegs = 24;
+static_assert(256 * kWorkRegs + 128 * kDoneRegs <= kTcThreads * 168, "register split");
 
 template <int D> struct TcCfg {
   static constexpr int NH = D / 64;                    // 128-byte column halves of a row
-  static constexpr uint32_t TILE = 128 * D * 2;        // Q of a chain, K or V of a tile
-  static constexpr int NK = D == 128 ? 3 : 6, NV = D == 128 ? 2 : 6;
-  static constexpr uint32_t OFF_K = 2 * TILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;
-  static constexpr uint32_t N_BARS = 2 * NK + 2 * NV + 2 * 4;
+  static constexpr uint32_t QTILE = 128 * D * 2;       // Q of a chain
+  static constexpr uint32_t TILE = TC_KT * D * 2;      // K or V of a tile
+  static constexpr int NK = D == 128 ? 5 : 12, NV = NK;
+  static constexpr uint32_t OFF_K = 2 * QTILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;
+  static constexpr uint32_t N_BARS = 2 * NK + 2 * NV + 14;
   static constexpr uint32_t SMEM = OFF_BAR + N_BARS * 8 + 16 + 1024;  // + alignment slack
   // afterwards the warps' rings, in the same bytes
   static constexpr int STAGES = (int)(OFF_BAR / kTcWarps / stage_bytes(D));
   static constexpr uint32_t RING = STAGES * stage_bytes(D);
   static_assert(plan_scratch(kPlanMax, kPlanMax) <= OFF_BAR, "the plan's scratch comes before all");
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
-  // tensor memory columns: S (and P) of the chains, O of the chains
+  // tensor memory columns: two S (and P) per chain, O of the chains
   static constexpr uint32_t COL_S = 0, COL_O = 256;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 32 bytes, a whole sector.
+__device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// One lane of the warp, in a form that the compiler knows for a single thread's:
+// its branch keeps the operands of the MMAs in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;}" : "=r"(p));
+  return p != 0;
+}
 
 struct TcParams {
   CUtensorMap tmap_k, tmap_v;  // 3-D [D, HKV, NB * BS] views, box {64, 1, 16}
@@ -121,10 +144,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   uint64_t* k_empty = k_full + NK;   // [NK] every S of it done
   uint64_t* v_full = k_empty + NK;   // [NV]
   uint64_t* v_empty = v_full + NV;   // [NV]
-  uint64_t* s_full = v_empty + NV;   // [2] a chain's S in tensor memory
-  uint64_t* p_full = s_full + 2;     // [2] its P written
-  uint64_t* o_ready = p_full + 2;    // [2] its P V done
-  uint64_t* q_ready = o_ready + 2;   // [2] its Q in shared memory
+  uint64_t* s_full = v_empty + NV;   // [2][2] S of a chain in tensor memory
+  uint64_t* p_full = s_full + 4;     // [2][2] its P written
+  uint64_t* o_ready = p_full + 4;    // [2] a chain's P V done
+  uint64_t* o_last = o_ready + 2;    // [2] its last P V of an item done
+  uint64_t* q_ready = o_last + 2;    // [2] its Q in shared memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   int32_t* abort_s = reinterpret_cast<int32_t*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -134,12 +158,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   // the scratch in shared memory, written and read as usual, is the TMA's next
   tc::fence_proxy_async_smem();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NK; ++s) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
-    for (int s = 0; s < NV; ++s) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+    for (int s = 0; s < NK; ++s) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 2);
+    for (int s = 0; s < NV; ++s) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 2);
+    for (int c = 0; c < 4; ++c) mbar_init(&s_full[c], 1), mbar_init(&p_full[c], 4);  // one arrival per warp
     for (int c = 0; c < 2; ++c) {
-      mbar_init(&s_full[c], 1);
-      mbar_init(&p_full[c], 4);  // one arrival per warp of the chain
       mbar_init(&o_ready[c], 1);
+      mbar_init(&o_last[c], 1);
       mbar_init(&q_ready[c], 4);
     }
     *abort_s = 0;
@@ -160,56 +184,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int c = warp >> 2, r = (warp & 3) * 32 + lane;  // chain, row of the chain = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t scol = C::COL_S + 128 * c, ocol = C::COL_O + 128 * c;
+    const uint32_t ocol = C::COL_O + 128 * c;
     // S is scaled by |qscale|; a negative scale is in Q's sign bits
     const float qs = fabsf(p.qscale);
     const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;
-    uint32_t uses = 0;  // tiles of this chain so far: the phase of its barriers
+    uint32_t uses = 0, done = 0;  // tiles, items with tiles of this chain: the phases of its barriers
     bool ok = true;
-    while (ok && walk.next(p, worker, im)) {
+    // Q of this thread's row of an item
+    uint4 qr[D / 8];
+    auto load_q = [&](const TcItem& it) {
+      const int row = it.rows <= 128 ? r : 128 * c + r, rr = it.r0 + row;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          static_cast<const T*>(p.q) + ((int64_t)(it.b0 + rr / p.G) * p.H + (int64_t)it.kvh * p.G + rr % p.G) * D);
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) qr[k] = row < it.rows ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+    };
+    bool more = walk.next(p, worker, im);
+    if (more) load_q(im);
+    while (more) {
       const bool by_keys = im.rows <= 128;
       const int row = by_keys ? r : 128 * c + r;  // of the unit
       const int tiles = by_keys ? (im.n - c + 1) / 2 : im.n;
       if (im.n > 0) {
-        unsigned char* qd = smem + c * C::TILE;
-        const int rr = im.r0 + row;
-        const bool in = row < im.rows;
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(p.q) +
-            ((int64_t)(im.b0 + rr / p.G) * p.H + (int64_t)im.kvh * p.G + rr % p.G) * D);
+        unsigned char* qd = smem + c * C::QTILE;
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          uint4 u = in ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
-          u.x ^= flip, u.y ^= flip, u.z ^= flip, u.w ^= flip;
-          *reinterpret_cast<uint4*>(qd + sw128_offset(r, 8 * k, 128)) = u;
-        }
+        for (int k = 0; k < D / 8; ++k)
+          *reinterpret_cast<uint4*>(qd + sw128_offset(r, 8 * k, 128)) =
+              make_uint4(qr[k].x ^ flip, qr[k].y ^ flip, qr[k].z ^ flip, qr[k].w ^ flip);
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_ready[c]);
       }
       float m_ref = -INFINITY, l = 0.f;
       for (int i = 0; i < tiles && ok; ++i, ++uses) {
-        if (!warp_wait_rx(&s_full[c], uses & 1, abort_s)) { ok = false; break; }
+        const uint32_t b = uses & 1, scol = lane_base + C::COL_S + 128 * c + 64 * b;
+        if (!warp_wait_rx(&s_full[2 * c + b], (uses >> 1) & 1, abort_s)) { ok = false; break; }
         tc::fence_after_sync();
-        const int j = im.j0 + (by_keys ? 2 * i + c : i);
-        const int lim = im.prefix - j * TC_KT;  // keys of the tile below the prefix's end
-        uint32_t u[128];
+        uint32_t u[64];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc::tmem_ld32(lane_base + scol + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * k));
+        for (int k = 0; k < 2; ++k) tc::tmem_ld32(scol + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(u + 32 * k));
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc::reg_fence(*reinterpret_cast<uint32_t(*)[32]>(u + 32 * k));
+        for (int k = 0; k < 2; ++k) tc::reg_fence(*reinterpret_cast<uint32_t(*)[32]>(u + 32 * k));
+        // keys of this tile below the prefix's end
+        const int lim = im.prefix - (im.j0 + (by_keys ? 2 * i + c : i)) * TC_KT;
         if (lim < TC_KT) {
 #pragma unroll
-          for (int k = 0; k < 128; ++k)
+          for (int k = 0; k < 64; ++k)
             if (k >= lim) u[k] = __float_as_uint(-INFINITY);
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < 128; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(u[k]));
+        for (int k = 0; k < 64; k += 2)
+          m4[k / 2 & 3] = max3(m4[k / 2 & 3], __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
         const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qs;
         // The reference only moves when the row's maximum grows by more than
         // 2^8; then O and l are rescaled (by 1 in rows that keep theirs)
@@ -224,21 +253,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
         const float2 neg2 = make_float2(neg, neg), qs2 = make_float2(qs, qs);
         float2 ls = make_float2(0.f, 0.f);
         // P = exp2(s - m_ref), keys 2k and 2k + 1 in column k
+        uint32_t w[32];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x = fma2(make_float2(__uint_as_float(u[32 * k + 2 * e]), __uint_as_float(u[32 * k + 2 * e + 1])), qs2, neg2);
-            const float2 y = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-            ls = add2(ls, y);
-            w[e] = pack2(y.x, y.y, (T*)nullptr);
-          }
-          tc::tmem_st16(lane_base + scol + 16 * k, w);
+        for (int e = 0; e < 32; ++e) {
+          const float2 x = fma2(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), qs2, neg2);
+          const float2 y = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          ls = add2(ls, y);
+          w[e] = pack2(y.x, y.y, (T*)nullptr);
         }
+        tc::tmem_st32(scol, w);
         l += ls.x + ls.y;
         if (rescale) {
-          // (the chain's previous P V must have finished)
+          // the chain's P V before this one must have finished (the one before
+          // that has: this S was issued after it)
           if (!warp_wait_rx(&o_ready[c], (uses - 1) & 1, abort_s)) { ok = false; break; }
           tc::fence_after_sync();
 #pragma unroll
@@ -254,14 +281,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
         tc::tmem_wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[c]);
+        if (lane == 0) mbar_arrive(&p_full[2 * c + b]);
       }
       // the piece's partials: (m_ref, l) and O as they are
-      if (ok && tiles > 0 && !warp_wait_rx(&o_ready[c], (uses - 1) & 1, abort_s)) ok = false;
+      // (the next item's Q comes meanwhile)
+      const TcItem cur = im;
+      more = ok && walk.next(p, worker, im);
+      if (more) load_q(im);
+      if (ok && tiles > 0 && !warp_wait_rx(&o_last[c], done++ & 1, abort_s)) ok = false;
       if (!ok) break;
       if (tiles > 0) tc::fence_after_sync();
-      const int64_t out = im.prow + (by_keys ? 128 * c + r : row);
-      const bool in = row < im.rows;
+      const int64_t out = cur.prow + (by_keys ? 128 * c + r : row);
+      const bool in = row < cur.rows;
       if (in) p.part_ml[out] = make_float2(m_ref, l);
       if (tiles > 0) {
         float* dst = p.part_o + out * D;
@@ -272,8 +303,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           tc::tmem_wait_ld();
           if (in) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(dst + 32 * k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 32; e += 8) store32(dst + 32 * k + e, o + e);
           }
         }
         // these reads come before the next unit's first P V, which follows P's arrival
@@ -284,70 +314,85 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     // Both chains done: every product has been taken, and the shared memory is
     // free for the rings of the warps' own work
     asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkRegs));
     if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
       warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, (int64_t)warp * gridDim.x + blockIdx.x);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kMmaWarp) {
-      // ------------------------------------------------------------ MMA issuer
+    if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+      // ------------------------------------ MMA issuer of chain `warp - kMmaWarp`
+      // A chain has two S, so that the next is there while the softmax works on
+      // this one: per tile P V, then S of the tile after next, which takes the
+      // place of P and waits for that P V to be done (products of different
+      // accumulators are not ordered by themselves).  Every tile is taken up
+      // and given back by both chains, so both follow its barriers' phases;
+      // with by_keys a chain passes over the other's tiles.
       constexpr uint32_t idesc_s = tc::idesc_f16(prefill::Fmt<T>::id, 128, TC_KT, false);
       constexpr uint32_t idesc_o = tc::idesc_f16(prefill::Fmt<T>::id, 128, D, true);
-      uint32_t k0 = 0, items = 0;       // tiles, items so far
-      uint32_t uses0 = 0, uses1 = 0;    // tiles of the chains so far
+      const int c = warp - kMmaWarp;
+      const uint64_t qd = tc::smem_desc_sw128(smem_u32(smem) + c * C::QTILE, 16, 1024);
+      const uint64_t kd = tc::smem_desc_sw128(smem_u32(smem) + C::OFF_K, 16, 1024);
+      const uint64_t vd = tc::smem_desc_sw128(smem_u32(smem) + C::OFF_V, TC_KT * 128, 1024);
+      const uint32_t scol = tmem + C::COL_S + 128 * c, ocol = tmem + C::COL_O + 128 * c;
+      uint32_t kn = 0, kp = 0, vn = 0, vp = 0;  // stage and phase of the coming K and V tile
+      uint32_t items = 0, ns = 0, np = 0;       // items; S and P V of this chain
       bool ok = true;
-      while (walk.next(p, worker, im)) {
-        if (lane != 0 || !ok || im.n == 0) continue;  // (the other lanes only walk along)
+      if (elect_one()) while (walk.next(p, worker, im)) {
+        if (!ok || im.n == 0) continue;
         const bool by_keys = im.rows <= 128;
-        // element e: chain e & 1 on tile e (by keys) or e / 2
-        const int E = by_keys ? im.n : 2 * im.n;
-        auto tile_of = [&](int e) -> uint32_t { return k0 + (by_keys ? e : e >> 1); };
-        auto issue_s = [&](int e) -> bool {
-          const int c = e & 1;
-          const uint32_t t = tile_of(e), st = t % NK;
-          if (e < 2 && !mbar_wait(&q_ready[c], items & 1, abort_s)) return false;
-          if (!mbar_wait(&k_full[st], (t / NK) & 1, abort_s)) return false;
-          tc::fence_after_sync();
-          const uint32_t qb = smem_u32(smem) + c * C::TILE, kb = smem_u32(smem) + C::OFF_K + st * C::TILE;
-          const uint32_t dcol = tmem + C::COL_S + 128 * c;
+        auto own = [&](int t) { return !by_keys || (t & 1) == c; };
+        int ts = 0, tv = 0, first = 1;  // tiles of the item whose S (P V) have been issued or passed over
+        // S of the chain's next tile, if there is one
+        auto start = [&](bool wait_pv) {
+          while (ts < im.n) {
+            if (!mbar_wait(&k_full[kn], kp, abort_s)) return false;
+            const bool mine = own(ts++);
+            if (mine) {
+              if (wait_pv && !mbar_wait(&o_ready[c], (np - 1) & 1, abort_s)) return false;
+              tc::fence_after_sync();
+              const uint64_t b = kd + (uint64_t)(kn * (C::TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-            tc::mma_ss(dcol, tc::smem_desc_sw128(qb + off, 16, 1024), tc::smem_desc_sw128(kb + off, 16, 1024), idesc_s,
-                       kk != 0);
+              for (int kk = 0; kk < D / 16; ++kk)
+                tc::mma_ss(scol + 64 * (ns & 1), qd + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4),
+                           b + (((kk >> 2) * (TC_KT * 128) + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+              tc::mma_commit(&s_full[2 * c + (ns & 1)]);
+              tc::mma_commit(&k_empty[kn]);
+              ++ns;
+            } else {
+              mbar_arrive(&k_empty[kn]);
+            }
+            if (++kn == NK) kn = 0, kp ^= 1;
+            if (mine) break;
           }
-          tc::mma_commit(&s_full[c]);
-          if (by_keys || c) tc::mma_commit(&k_empty[st]);
           return true;
         };
-        ok = issue_s(0);
-        if (ok && E > 1) ok = issue_s(1);
-        for (int e = 0; e < E && ok; ++e) {
-          const int c = e & 1;
-          const uint32_t t = tile_of(e), st = t % NV, uses = c ? uses1 : uses0;
-          if (!mbar_wait(&v_full[st], (t / NV) & 1, abort_s) || !mbar_wait(&p_full[c], uses & 1, abort_s)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
-          const uint32_t vb = smem_u32(smem) + C::OFF_V + st * C::TILE;
-          const uint32_t pcol = tmem + C::COL_S + 128 * c, dcol = tmem + C::COL_O + 128 * c;
+        ok = mbar_wait(&q_ready[c], items & 1, abort_s) && start(false) && start(false);
+        while (tv < im.n && ok) {
+          if (!mbar_wait(&v_full[vn], vp, abort_s)) { ok = false; break; }
+          const bool mine = own(tv++);
+          if (mine) {
+            if (!mbar_wait(&p_full[2 * c + (np & 1)], (np >> 1) & 1, abort_s)) { ok = false; break; }
+            tc::fence_after_sync();
+            const uint64_t b = vd + (uint64_t)(vn * (C::TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < TC_KT / 16; ++kk)  // 16 keys: 8 columns of pairs
-            tc::mma_ts(dcol, pcol + kk * 8, tc::smem_desc_sw128(vb + kk * 16 * 128, 128 * 128, 1024), idesc_o,
-                       (e > 1 || kk > 0) ? 1u : 0u);
-          if (by_keys || c) tc::mma_commit(&v_empty[st]);
-          tc::mma_commit(&o_ready[c]);
-          if (c) ++uses1;
-          else ++uses0;
-          if (e + 2 < E) ok = issue_s(e + 2);
+            for (int kk = 0; kk < TC_KT / 16; ++kk)  // 16 keys: 8 columns of pairs
+              tc::mma_ts(ocol, scol + 64 * (np & 1) + kk * 8, b + (uint64_t)(kk * 128), idesc_o, kk > 0 || !first);
+            first = 0;
+            ++np;
+            tc::mma_commit(&o_ready[c]);
+            if (tv + (by_keys ? 1 : 0) >= im.n) tc::mma_commit(&o_last[c]);
+            tc::mma_commit(&v_empty[vn]);
+          } else {
+            mbar_arrive(&v_empty[vn]);
+          }
+          if (++vn == NV) vn = 0, vp ^= 1;
+          if (mine) ok = start(true);
         }
         if (!ok) report(p.dev_status, PA_DEVERR_TIMEOUT);
-        k0 += im.n;
         ++items;
       }
     } else if (warp == kKWarp || warp == kVWarp) {
       // ---------------------------------------------------- K and V producers
-      // Lane l < 8 NH loads one 16-row group x 64-column half of a tile; its
+      // Lane l < 4 NH loads one 16-row group x 64-column half of a tile; its
       // block id is fetched a tile ahead.
       const bool is_v = warp == kVWarp;
       const int n_st = is_v ? NV : NK;
@@ -355,7 +400,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       uint64_t* empty = is_v ? v_empty : k_empty;
       unsigned char* base = smem + (is_v ? C::OFF_V : C::OFF_K);
       const CUtensorMap* map = is_v ? &tp.tmap_v : &tp.tmap_k;
-      constexpr int NBOX = 8 * C::NH;
+      constexpr int NBOX = TC_KT / 16 * C::NH;
       const int g16 = lane / C::NH, hf = lane % C::NH;
       const int32_t BS = (int32_t)p.BS;
       uint32_t n = 0;
@@ -381,7 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           if (i + 1 < im.n) next_row = row_of(j + 1);
           const uint32_t st = n % n_st;
           if (!warp_wait(&empty[st], ((n / n_st) & 1) ^ 1, abort_s)) { ok = false; break; }
-          unsigned char* dst = base + st * C::TILE + hf * (128 * 128) + g16 * 16 * 128;
+          unsigned char* dst = base + st * C::TILE + hf * (TC_KT * 128) + g16 * 16 * 128;
           // a V group that reaches past the prefix is written by its lane, its
           // rows past the end as zeros; a K group there loads any row (its
           // scores are masked)
@@ -405,6 +450,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           (void)mbar_wait(&full[i % n_st], (i / n_st) & 1);
       }
     }
+    __syncwarp();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDoneRegs));
   }
 
   tc::fence_before_sync();
