@@ -71,9 +71,17 @@ struct Params {
 
 __host__ __device__ __forceinline__ int32_t cdiv(int32_t a, int32_t b) { return (a + b - 1) / b; }
 
-// Worker w's first tile, and the worker of tile x, for T tiles over W workers.
-__device__ __forceinline__ int64_t first_tile(int64_t w, int64_t T, int64_t W) { return w * T / W; }
-__device__ __forceinline__ int64_t worker_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W - 1) / T; }
+// Worker w's first tile, and the worker of tile x, for T tiles over W workers
+// (in 32 bits where that holds the products: the division is several times
+// shorter, and stands in the way of a call's first loads).
+__device__ __forceinline__ int64_t first_tile(int64_t w, int64_t T, int64_t W) {
+  if ((w | W) < 0x10000 && T < 0x10000) return (uint32_t)w * (uint32_t)T / (uint32_t)W;
+  return w * T / W;
+}
+__device__ __forceinline__ int64_t worker_of(int64_t x, int64_t T, int64_t W) {
+  if (T < 0x10000 && W < 0x10000) return ((uint32_t)(x + 1) * (uint32_t)W - 1) / (uint32_t)T;
+  return ((x + 1) * W - 1) / T;
+}
 
 // One of the structs above, in 16-byte loads.
 template <typename E> __device__ __forceinline__ E load_plan(const E* e) {

@@ -40,6 +40,13 @@ constexpr int kTcThreads = 384;
 constexpr int kWorkRegs = 240, kDoneRegs = 24;
 static_assert(256 * kWorkRegs + 128 * kDoneRegs <= kTcThreads * 168, "register split");
 
+// A warp's bounded wait on a barrier that hands tensor-memory data on, usually
+// passed at once.
+__device__ __forceinline__ bool wait_tmem(uint64_t* bar, uint32_t parity, int32_t* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_rx(bar, parity, 0u))) return true;
+  return warp_wait_rx(bar, parity, abort_flag);
+}
+
 template <int D> struct TcCfg {
   static constexpr int NH = D / 64;                    // 128-byte column halves of a row
   static constexpr uint32_t QTILE = 128 * D * 2;       // Q of a chain
@@ -180,7 +187,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   const Totals tot = load_plan(plan.totals);
   const int64_t worker = blockIdx.x;
   Walk walk(p, plan, tot, worker, lane);
-  TcItem im;
+  TcItem im = {};
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
@@ -192,17 +199,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;
     uint32_t uses = 0, done = 0;  // tiles, items with tiles of this chain: the phases of its barriers
     bool ok = true;
-    // Q of this thread's row of an item
+    // Q of this thread's row of an item (zeros for none: written in any case, so
+    // that it takes no registers while the tiles are worked on)
     uint4 qr[D / 8];
-    auto load_q = [&](const TcItem& it) {
+    auto load_q = [&](const TcItem& it, bool there) {
       const int row = it.rows <= 128 ? r : 128 * c + r, rr = it.r0 + row;
       const uint4* src = reinterpret_cast<const uint4*>(
           static_cast<const T*>(p.q) + ((int64_t)(it.b0 + rr / p.G) * p.H + (int64_t)it.kvh * p.G + rr % p.G) * D);
 #pragma unroll
-      for (int k = 0; k < D / 8; ++k) qr[k] = row < it.rows ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < D / 8; ++k) qr[k] = there && row < it.rows ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
     };
     bool more = walk.next(p, worker, im);
-    if (more) load_q(im);
+    load_q(im, more);
     while (more) {
       const bool by_keys = im.rows <= 128;
       const int row = by_keys ? r : 128 * c + r;  // of the unit
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       float m_ref = -INFINITY, l = 0.f;
       for (int i = 0; i < tiles && ok; ++i, ++uses) {
         const uint32_t b = uses & 1, scol = lane_base + C::COL_S + 128 * c + 64 * b;
-        if (!warp_wait_rx(&s_full[2 * c + b], (uses >> 1) & 1, abort_s)) { ok = false; break; }
+        if (!wait_tmem(&s_full[2 * c + b], (uses >> 1) & 1, abort_s)) { ok = false; break; }
         tc::fence_after_sync();
         uint32_t u[64];
 #pragma unroll
@@ -287,7 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       // (the next item's Q comes meanwhile)
       const TcItem cur = im;
       more = ok && walk.next(p, worker, im);
-      if (more) load_q(im);
+      load_q(im, more);
       if (ok && tiles > 0 && !warp_wait_rx(&o_last[c], done++ & 1, abort_s)) ok = false;
       if (!ok) break;
       if (tiles > 0) tc::fence_after_sync();
