@@ -23,10 +23,11 @@
 namespace pa {
 namespace shared {
 
-// The plan as a launch of its own, for more sequences or groups than kPlanMax.
+// The plan as a launch of its own, for more sequences or groups than kPlanMax
+// and for counts past 32 bits.
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
-  make_plan(p, plan_at(p, 0), p.plan + p.scratch_off, true);
+  make_plan<long long>(p, plan_at(p, 0), p.plan + p.scratch_off, true);
 }
 
 // All of the work by warps: pools that the tensor-memory part does not load.
@@ -117,26 +118,34 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= alpha;
     const uint32_t read = __ballot_sync(0xffffffffu, !none);
-#pragma unroll 8
-    for (int c = 0; c < min(32, n - c0); ++c) {
-      const float wc = __shfl_sync(0xffffffffu, w, c);
-      const float* src = p.part_o + piece(c0 + c) * D + lane * V;
-      float x[E];
+    // eight pieces' loads at a time, in any case (past the last the last again)
+    constexpr int K = D == 256 ? 4 : 8;
+    const int cnt = min(32, n - c0);
+    for (int c = 0; c < cnt; c += K) {
+      float x[K][E];
 #pragma unroll
-      for (int i = 0; i < E / V; ++i) {
-        if constexpr (V == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
-          x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
-        } else if constexpr (V == 2) {
-          const float2 f = *reinterpret_cast<const float2*>(src);
-          x[0] = f.x, x[1] = f.y;
-        } else {
-          x[0] = *src;
+      for (int k = 0; k < K; ++k) {
+        const float* src = p.part_o + piece(c0 + min(c + k, cnt - 1)) * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < E / V; ++i) {
+          if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
+            x[k][4 * i] = f.x, x[k][4 * i + 1] = f.y, x[k][4 * i + 2] = f.z, x[k][4 * i + 3] = f.w;
+          } else if constexpr (V == 2) {
+            const float2 f = *reinterpret_cast<const float2*>(src);
+            x[k][0] = f.x, x[k][1] = f.y;
+          } else {
+            x[k][0] = *src;
+          }
         }
       }
-      const bool in = read >> c & 1;  // (loaded in any case, so that the loads need not wait for ml)
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(wc, in ? x[e] : 0.f, acc[e]);
+      for (int k = 0; k < K; ++k) {
+        const float wc = __shfl_sync(0xffffffffu, w, min(c + k, 31));
+        const bool in = c + k < cnt && (read >> (c + k) & 1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(in ? wc : 0.f, in ? x[k][e] : 0.f, acc[e]);
+      }
     }
   }
   // no key, or only scores of -inf: L = 0, so out is NaN and lse -inf
@@ -175,7 +184,8 @@ static int warps_per_cta(int64_t D) {
 // rows each, for sequences' own units with min(G, ROWS), for the tensor
 // memory's with TC_ROWS.  `tc`: whether this launch has that part (a size query,
 // which does not know the pool, assumes the larger).
-static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, bool tc, Layout* y) {
+static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, bool tc, int64_t max_ctx,
+                  Layout* y) {
   const int64_t G = H / HKV;
   y->tc = tc && NG && B * G >= kTcRows && (D == 64 || D == 128);
   y->warps = (int64_t)sms * (y->tc ? kTcWarps : warps_per_cta(D));
@@ -187,7 +197,9 @@ static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int 
   if (y->tc) rows += (HKV * (B * G / TC_ROWS + std::min<int64_t>(NG, B * G / kTcRows)) + sms) * TC_ROWS;
   if (rows >= (int64_t(1) << 31) || B * H >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
-  y->planned = B > kPlanMax || NG > kPlanMax;
+  // tiles of every unit if all had the longest context
+  const double most_tiles = (double)(pre_units + own_units) * ((double)max_ctx / KT + 1 + kTcUnitCost);
+  y->planned = B > kPlanMax || NG > kPlanMax || most_tiles >= 2147483647.0;
   y->group_off = 256;
   y->seq_off = y->group_off + up(NG * (int64_t)sizeof(Group));
   y->scratch_off = y->seq_off + up(B * (int64_t)sizeof(Seq));
@@ -265,9 +277,13 @@ extern "C" int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, in
   int sms = 0;
   if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
   shared::Layout y;
-  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, true, &y);
+  // for either place of the plan
+  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, true, 0, &y);
   if (st) return st;
   *bytes = y.total;
+  st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms, true, int64_t(1) << 62, &y);
+  if (st) return st;
+  *bytes = std::max(*bytes, y.total);
   return PA_OK;
 }
 
@@ -298,7 +314,7 @@ extern "C" int pa_paged_attention_shared(
   if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
   shared::Layout y;
   st = shared::layout(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, sms,
-                      shared::tc_takes(head_dim, block_size, num_blocks), &y);
+                      shared::tc_takes(head_dim, block_size, num_blocks), block_size * max_blocks, &y);
   if (st) return st;
   if (!workspace || workspace_bytes < y.total) return PA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PA_ERR_ALIGNMENT;

@@ -126,9 +126,9 @@ __device__ __forceinline__ Plan plan_at(const Params& p, int64_t copy) {
 }
 
 // Sequences and groups up to which every CTA makes the plan itself, in shared
-// memory: one launch less, which small calls notice.
+// memory, if its counts fit 32 bits: one launch less, which small calls notice.
 constexpr int kPlanMax = 1024;
-constexpr int64_t kScanBytes = 2 * 32 * 32 + 16;  // the scans' sums, a counter
+constexpr int64_t kScanBytes = 2 * 32 * 40 + 16;  // the scans' sums, a counter
 __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
   return kScanBytes + (2 * B + 3 * (NG + 1)) * 4;
 }
@@ -150,44 +150,46 @@ __host__ __device__ __forceinline__ int32_t tc_unit_tiles(int32_t keys) {
   return keys ? cdiv(keys, TC_KT) + kTcUnitCost : 0;
 }
 
-// Exclusive scan of N values over the block on top of the running totals
+// Exclusive scan of N counts over the block on top of the running totals
 // `base`; warp_sums: one entry a warp, not in use by an earlier scan any more.
-template <int N> struct Sums {
-  long long v[N];
+// I: 32 bits where the host knows that the counts fit.
+template <typename I, int N> struct Sums {
+  I v[N];
 };
-template <int N>
-__device__ __forceinline__ Sums<N> block_scan(const Sums<N>& x, Sums<N>* warp_sums, Sums<N>& base) {
+template <typename I, int N>
+__device__ __forceinline__ Sums<I, N> block_scan(const Sums<I, N>& x, Sums<I, N>* warp_sums, Sums<I, N>& base) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  Sums<N> s = x;
+  auto warp_scan = [&](Sums<I, N> s) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
+    for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const long long y = __shfl_up_sync(0xffffffffu, s.v[i], o);
-      if (lane >= o) s.v[i] += y;
-    }
+      for (int i = 0; i < N; ++i) {
+        const I y = __shfl_up_sync(0xffffffffu, s.v[i], o);
+        if (lane >= o) s.v[i] += y;
+      }
+    return s;
+  };
+  const Sums<I, N> s = warp_scan(x);
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  Sums<N> r = {}, all = {};
-  for (int w = 0; w < warps; ++w)  // at most 32, the same words for all lanes
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (w < warp) r.v[i] += warp_sums[w].v[i];
-      all.v[i] += warp_sums[w].v[i];
-    }
+  const Sums<I, N> all = warp_scan(lane < warps ? warp_sums[lane] : Sums<I, N>{});
+  Sums<I, N> r;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    r.v[i] += base.v[i] + s.v[i] - x.v[i];
-    base.v[i] += all.v[i];
+    const I before = __shfl_sync(0xffffffffu, all.v[i], max(warp - 1, 0));
+    r.v[i] = base.v[i] + (warp ? before : 0) + s.v[i] - x.v[i];
+    base.v[i] += __shfl_sync(0xffffffffu, all.v[i], 31);
   }
   return r;
 }
 
 // One CTA makes the plan; `scratch`: plan_scratch() bytes, in shared memory or
 // its own part of the workspace.  Ends with a barrier.
+template <typename I>
 __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void* scratch, bool tell) {
-  auto sums = static_cast<Sums<4>(*)[32]>(scratch);
-  unsigned long long& tc_work = *reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + 2 * 32 * 32);
+  using S = Sums<I, 5>;
+  auto sums = static_cast<S(*)[32]>(scratch);
+  unsigned long long& tc_work = *reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + 2 * 32 * 40);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
   const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
@@ -233,34 +235,32 @@ __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void
   }
   __syncthreads();
   const bool use_tc = p.tc_rows && tc_work >= (unsigned long long)kTcMinTiles * p.tc_ctas;
-  // running counts: of the groups' tiles (the warps', the tensor memory's) and
-  // units (the tensor memory's in the high half), and of the sequences' tiles
-  Sums<4> base = {};
+  // running counts: the groups' tiles and units (the warps', the tensor
+  // memory's), the sequences' tiles
+  S base = {};
   for (int32_t i0 = 0, k = 0; i0 < max(B, groups); i0 += threads, k ^= 1) {
     const int32_t i = i0 + tid;
-    Sums<4> x = {};
+    S x = {};
     int32_t n = 0, prefix = 0, tc = 0, from = 0, g = -1;
     if (i < groups) {
       n = gs[i + 1] - gs[i];
       prefix = pre[i];
       tc = use_tc && n * G >= p.tc_rows;
-      const long long units = (long long)HKV * cdiv(n * G, tc ? TC_ROWS : ROWS);
-      x = tc ? Sums<4>{{0, units * tc_unit_tiles(prefix), units << 32, 0}}
-             : Sums<4>{{units * unit_tiles(prefix), 0, units, 0}};
+      const I units = (I)HKV * cdiv(n * G, tc ? TC_ROWS : ROWS);
+      x = tc ? S{{0, units * tc_unit_tiles(prefix), 0, units, 0}} : S{{units * unit_tiles(prefix), 0, units, 0, 0}};
     }
     if (i < B) {
       g = grp[i];
       if (g >= 0) from = min(pre[g], ctx[i]);
-      x.v[3] = (long long)HKV * cdiv(G, ROWS) * unit_tiles(ctx[i] - from);
+      x.v[4] = (I)HKV * cdiv(G, ROWS) * unit_tiles(ctx[i] - from);
     }
-    const Sums<4> at = block_scan(x, sums[k], base);
+    const S at = block_scan(x, sums[k], base);
     if (i < groups)
-      out.groups[i] = Group{{at.v[0], at.v[1]}, gs[i], n, lead[i], prefix,
-                            {(int32_t)(at.v[2] & 0xffffffff), (int32_t)(at.v[2] >> 32)}, tc, 0};
-    if (i < B) out.seqs[i] = Seq{{at.v[3]}, from, ctx[i], g, 0};
+      out.groups[i] = Group{{at.v[0], at.v[1]}, gs[i], n, lead[i], prefix, {(int32_t)at.v[2], (int32_t)at.v[3]}, tc, 0};
+    if (i < B) out.seqs[i] = Seq{{at.v[4]}, from, ctx[i], g, 0};
   }
   if (tid == 0) {
-    const int64_t tiles = base.v[0] + base.v[3], tc_tiles = base.v[1];
+    const int64_t tiles = (int64_t)base.v[0] + base.v[4], tc_tiles = base.v[1];
     *out.totals = Totals{base.v[0], tiles, min((int64_t)p.warps, max((tiles + kMinTiles - 1) / kMinTiles, (int64_t)1)),
                          tc_tiles, min((int64_t)p.tc_ctas, max(tc_tiles, (int64_t)1))};
   }
@@ -274,7 +274,7 @@ __device__ __forceinline__ Plan take_plan(const Params& p, void* smem_scratch) {
     return plan_at(p, 0);
   }
   const Plan plan = plan_at(p, blockIdx.x);
-  make_plan(p, plan, smem_scratch, blockIdx.x == 0);
+  make_plan<int32_t>(p, plan, smem_scratch, blockIdx.x == 0);
   return plan;
 }
 
