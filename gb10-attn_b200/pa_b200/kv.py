@@ -345,6 +345,56 @@ class TorchBlockAllocator:
             outs.append(ops.decode_layer_step(q_layers[layer], kc, vc, bt, ctx, sc, kn, vn))
         return torch.stack(outs)
 
+    # -- sequences that share pages -----------------------------------------------
+    def prefix_groups(self, allocations) -> tuple[torch.Tensor, torch.Tensor]:
+        """(group_starts [NG + 1], prefix_lens [NG]) of a batch for
+        ``ops.paged_attention_shared``: neighbours in the batch that start with
+        the same block form a group, and its prefix is the blocks that all of
+        them start with (forks of one parent side by side share its full
+        pages).  int32 on the pool's device; valid until the batch changes."""
+        starts, lens = [0], []
+        i = 0
+        while i < len(allocations):
+            first = allocations[i].block_ids
+            n, j = len(first), i + 1
+            while j < len(allocations) and first and allocations[j].block_ids[:1] == first[:1]:
+                other = allocations[j].block_ids
+                n = next((k for k in range(min(n, len(other))) if other[k] != first[k]),
+                         min(n, len(other)))
+                j += 1
+            lens.append(min([n * self.kv_cfg.block_size] +
+                            [a.num_tokens for a in allocations[i:j]]))
+            starts.append(j)
+            i = j
+
+        def dev(x):
+            return torch.tensor(x, dtype=torch.int32).to(self.device)
+
+        return dev(starts), dev(lens)
+
+    def layer_step_shared(self, layer: int, q, k, v, q_weight, k_weight, cos_sin, positions,
+                          block_tables, context_lens, group_starts, prefix_lens,
+                          eps: float = 1e-6, scale: float | None = None,
+                          interleaved: bool = False):
+        """One layer of a decode step for sequences that share prefixes: the
+        new tokens' q and k normalised and rotated, k and v appended
+        (``ops.qk_norm_rope_append``), then the attention with each prefix read
+        once for its group (``ops.paged_attention_shared``).
+
+        q [B, n_head, head_dim], k, v [B, n_kv_head, head_dim] of the pool's
+        type (fp16 or bf16), strided parts of one projection allowed;
+        positions[b] is where sequence b's token goes (negative: idle),
+        context_lens[b] counts it.  Returns [B, n_head, head_dim]."""
+        from . import ops
+        none = torch.empty(0, device=self.device)
+        kc, vc = self.layer_kv(layer)
+        q = ops.qk_norm_rope_append(q, k, v, none if q_weight is None else q_weight,
+                                    none if k_weight is None else k_weight, eps, cos_sin,
+                                    interleaved, positions, none, kc, vc, block_tables, none, none)
+        sc = q.shape[-1] ** -0.5 if scale is None else float(scale)
+        return ops.paged_attention_shared(q, kc, vc, block_tables, context_lens, group_starts,
+                                          prefix_lens, sc)[0]
+
     # -- writer ----------------------------------------------------------------
     _IDS_CACHE_MAX = 4096
 
