@@ -62,48 +62,40 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= p.B * p.H) return;
-  const int64_t b = row / p.H;
-  const int32_t h = (int32_t)(row % p.H), kv = h / p.G, g = h % p.G;
-  const int32_t own_y = cdiv(p.G, ROWS), own_rows = min(p.G, ROWS);
-  const Plan plan = plan_at(p, 0);
-  const Totals tot = load_plan(plan.totals);
-  const Seq sp = load_plan(plan.seqs + b);
-  // this row's pieces: first of its prefix unit, pre_step rows apart, then of its own
-  int64_t pre0 = 0, own0 = 0;
-  int32_t n_pre = 0, n_own = 0, pre_step = 0;
-  if (sp.group >= 0 && sp.from > 0) {
-    const Group gp = load_plan(plan.groups + sp.group);
-    const int32_t rows = gp.n * p.G, r = ((int32_t)b - gp.b0) * p.G + g;
-    const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R);
-    const int32_t nt = gp.tc ? tc_unit_tiles(gp.prefix) : unit_tiles(gp.prefix);
-    const int64_t tiles = gp.tc ? tot.tc_tiles : tot.tiles, workers = gp.tc ? tot.tc_workers : tot.workers;
-    const int32_t u = kv * ry + r / R;
-    const int64_t a = (gp.tc ? gp.tile0[1] : gp.tile0[0]) + (int64_t)u * nt;
-    const int64_t w0 = worker_of(a, tiles, workers);
-    n_pre = (int32_t)(worker_of(a + nt - 1, tiles, workers) - w0) + 1;
-    pre0 = (gp.tc ? p.tc_row0 : 0) + ((gp.tc ? gp.unit0[1] : gp.unit0[0]) + u + w0) * R + r % R;
-    pre_step = R;
-    // a unit of at most 128 rows: a piece from each chain
-    if (gp.tc && rows - r / R * R <= R / 2) pre_step = R / 2, n_pre *= 2;
-  }
-  if (sp.ctx > sp.from) {
-    const int32_t nt = unit_tiles(sp.ctx - sp.from), u = kv * own_y + g / ROWS;
-    const int64_t a = tot.prefix_tiles + sp.tile0[0] + (int64_t)u * nt;
-    const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
-    n_own = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
-    own0 = p.own_row0 + (b * p.HKV * own_y + u + w0) * own_rows + g % ROWS;
-  }
+  const Pieces at = load_plan(p.pieces + row);
+  const int32_t own_rows = min(p.G, ROWS), n_pre = at.n_pre, n_own = at.n_own;
   const int n = n_pre + n_own;
   auto piece = [&](int c) -> int64_t {
-    return c < n_pre ? pre0 + (int64_t)c * pre_step : own0 + (int64_t)(c - n_pre) * own_rows;
+    return c < n_pre ? at.pre0 + (int64_t)c * at.pre_step : at.own0 + (int64_t)(c - n_pre) * own_rows;
   };
   // 32 pieces at a time, lane c with the maximum and sum of piece c; then their
   // O, several in flight
   constexpr int V = D >= 128 ? 4 : D / 32;  // elements per load
   float acc[E] = {}, L = 0.f, M = -INFINITY;
+  constexpr int K = D == 256 ? 4 : 8;
+  float x[K][E];
+  auto fetch = [&](int c) {  // O of K pieces from c on (past the last the last again)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float* src = p.part_o + piece(min(c + k, n - 1)) * D + lane * V;
+#pragma unroll
+      for (int i = 0; i < E / V; ++i) {
+        if constexpr (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
+          x[k][4 * i] = f.x, x[k][4 * i + 1] = f.y, x[k][4 * i + 2] = f.z, x[k][4 * i + 3] = f.w;
+        } else if constexpr (V == 2) {
+          const float2 f = *reinterpret_cast<const float2*>(src);
+          x[k][0] = f.x, x[k][1] = f.y;
+        } else {
+          x[k][0] = *src;
+        }
+      }
+    }
+  };
   for (int c0 = 0; c0 < n; c0 += 32) {
     float2 ml = make_float2(-INFINITY, 0.f);
     if (c0 + lane < n) ml = p.part_ml[piece(c0 + lane)];
+    fetch(c0);
     const bool none = ml.x == -INFINITY && ml.y == 0.f;  // without keys, or only scores of -inf: O not used
     float top = ml.x;
 #pragma unroll
@@ -117,32 +109,14 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
     L = fmaf(L, alpha, l);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= alpha;
-    const uint32_t read = __ballot_sync(0xffffffffu, !none);
-    // eight pieces' loads at a time, in any case (past the last the last again)
-    constexpr int K = D == 256 ? 4 : 8;
+    const uint32_t used = __ballot_sync(0xffffffffu, !none);
     const int cnt = min(32, n - c0);
     for (int c = 0; c < cnt; c += K) {
-      float x[K][E];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const float* src = p.part_o + piece(c0 + min(c + k, cnt - 1)) * D + lane * V;
-#pragma unroll
-        for (int i = 0; i < E / V; ++i) {
-          if constexpr (V == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + i * 128);
-            x[k][4 * i] = f.x, x[k][4 * i + 1] = f.y, x[k][4 * i + 2] = f.z, x[k][4 * i + 3] = f.w;
-          } else if constexpr (V == 2) {
-            const float2 f = *reinterpret_cast<const float2*>(src);
-            x[k][0] = f.x, x[k][1] = f.y;
-          } else {
-            x[k][0] = *src;
-          }
-        }
-      }
+      if (c) fetch(c0 + c);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const float wc = __shfl_sync(0xffffffffu, w, min(c + k, 31));
-        const bool in = c + k < cnt && (read >> (c + k) & 1);
+        const bool in = c + k < cnt && (used >> (c + k) & 1);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(in ? wc : 0.f, in ? x[k][e] : 0.f, acc[e]);
       }
@@ -173,7 +147,7 @@ constexpr int kTcRows = 33;
 struct Layout {
   bool tc, planned;
   int64_t warps, plan_bytes, group_off, seq_off, scratch_off, own_row0, tc_row0;
-  size_t ml, o, total;
+  size_t pieces, ml, o, total;
 };
 
 static int warps_per_cta(int64_t D) {
@@ -204,7 +178,8 @@ static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int 
   y->seq_off = y->group_off + up(NG * (int64_t)sizeof(Group));
   y->scratch_off = y->seq_off + up(B * (int64_t)sizeof(Seq));
   y->plan_bytes = y->scratch_off + (y->planned ? up(plan_scratch(B, NG)) : 0);
-  y->ml = (size_t)(y->plan_bytes * (y->planned ? 1 : sms));
+  y->pieces = (size_t)(y->plan_bytes * (y->planned ? 1 : sms));
+  y->ml = y->pieces + (size_t)up(B * H * (int64_t)sizeof(Pieces));
   y->o = y->ml + (size_t)up(rows * (int64_t)sizeof(float2));
   y->total = y->o + (size_t)up(rows * D * (int64_t)sizeof(float));
   return PA_OK;
@@ -352,6 +327,7 @@ extern "C" int pa_paged_attention_shared(
   p.tc_row0 = y.tc_row0;
   p.tc_rows = y.tc ? shared::kTcRows : 0;
   p.tc_ctas = sms;
+  p.pieces = reinterpret_cast<shared::Pieces*>(ws + y.pieces);
   p.part_ml = reinterpret_cast<float2*>(ws + y.ml);
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.dev_status = dev_status;

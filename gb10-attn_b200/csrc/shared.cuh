@@ -45,6 +45,13 @@ struct alignas(16) Totals {
   int64_t tc_tiles, tc_workers;          // the tensor memory's
 };
 
+// Where the partials of an output row are: n_pre pieces of its prefix unit,
+// pre_step rows apart, and n_own of its own.
+struct alignas(16) Pieces {
+  int64_t pre0, own0;
+  int32_t n_pre, n_own, pre_step, pad;
+};
+
 struct Params {
   void* out;
   float* lse;  // [B, H]
@@ -60,6 +67,7 @@ struct Params {
   int64_t plan_bytes;   // bytes of one
   int64_t group_off, seq_off, scratch_off;  // its groups, sequences, scratch (made by plan_kernel only)
   int32_t planned;      // a launch of its own makes the plan
+  Pieces* pieces;       // [B, H]
   float2* part_ml;  // (running max in log2 units, sum)
   float* part_o;
   int64_t own_row0; // first partial row of the sequences' own units
@@ -402,6 +410,46 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half*) {
 // One stage of a warp's ring: the K rows of a tile, then its V rows.
 __host__ __device__ constexpr uint32_t stage_bytes(int D) { return 2 * KT * D * 2; }
 
+// The pieces of output row `row`.
+__device__ __forceinline__ Pieces locate(const Params& p, const Plan& plan, const Totals& tot, int64_t row) {
+  const int64_t b = row / p.H;
+  const int32_t h = (int32_t)(row % p.H), kv = h / p.G, g = h % p.G;
+  const int32_t own_y = cdiv(p.G, ROWS), own_rows = min(p.G, ROWS);
+  const Seq sp = load_plan(plan.seqs + b);
+  int64_t pre0 = 0, own0 = 0;
+  int32_t n_pre = 0, n_own = 0, pre_step = 0;
+  if (sp.group >= 0 && sp.from > 0) {
+    const Group gp = load_plan(plan.groups + sp.group);
+    const int32_t rows = gp.n * p.G, r = ((int32_t)b - gp.b0) * p.G + g;
+    const int32_t R = gp.tc ? TC_ROWS : ROWS, ry = cdiv(rows, R);
+    const int32_t nt = gp.tc ? tc_unit_tiles(gp.prefix) : unit_tiles(gp.prefix);
+    const int64_t tiles = gp.tc ? tot.tc_tiles : tot.tiles, workers = gp.tc ? tot.tc_workers : tot.workers;
+    const int32_t u = kv * ry + r / R;
+    const int64_t a = (gp.tc ? gp.tile0[1] : gp.tile0[0]) + (int64_t)u * nt;
+    const int64_t w0 = worker_of(a, tiles, workers);
+    n_pre = (int32_t)(worker_of(a + nt - 1, tiles, workers) - w0) + 1;
+    pre0 = (gp.tc ? p.tc_row0 : 0) + ((gp.tc ? gp.unit0[1] : gp.unit0[0]) + u + w0) * R + r % R;
+    pre_step = R;
+    // a unit of at most 128 rows: a piece from each chain
+    if (gp.tc && rows - r / R * R <= R / 2) pre_step = R / 2, n_pre *= 2;
+  }
+  if (sp.ctx > sp.from) {
+    const int32_t nt = unit_tiles(sp.ctx - sp.from), u = kv * own_y + g / ROWS;
+    const int64_t a = tot.prefix_tiles + sp.tile0[0] + (int64_t)u * nt;
+    const int64_t w0 = worker_of(a, tot.tiles, tot.workers);
+    n_own = (int32_t)(worker_of(a + nt - 1, tot.tiles, tot.workers) - w0) + 1;
+    own0 = p.own_row0 + (b * p.HKV * own_y + u + w0) * own_rows + g % ROWS;
+  }
+  return {pre0, own0, n_pre, n_own, pre_step, 0};
+}
+
+// A worker's share of the rows, for the merge.  Every worker of the launch calls
+// it, with work or without.
+__device__ __forceinline__ void locate_rows(const Params& p, const Plan& plan, const Totals& tot, int64_t worker) {
+  for (int64_t r = worker * 32 + (threadIdx.x & 31); r < p.B * p.H; r += (int64_t)p.warps * 32)
+    p.pieces[r] = locate(p, plan, tot, r);
+}
+
 // A warp streams its items through a ring of its own: for each the rows of Q,
 // then tile after tile the rows of K and V (16-byte asynchronous copies, so any
 // page size and any first token serve).  The copies run NST - 1 stages ahead
@@ -505,6 +553,9 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
     fill(st_ld, k, r);
     step(st_ld);
   };
+
+  // While the first bytes are on their way
+  locate_rows(p, plan, tot, worker);
 
   // ---- the products' side
   const int mi = lane >> 3, mr = lane & 7;  // matrix and row that this lane addresses

@@ -323,8 +323,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     // free for the rings of the warps' own work
     asm volatile("bar.sync 1, 256;" ::: "memory");
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkRegs));
+    const int64_t own = (int64_t)warp * gridDim.x + blockIdx.x;
     if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
-      warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, (int64_t)warp * gridDim.x + blockIdx.x);
+      warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, own);
+    else
+      locate_rows(p, plan, tot, own);  // the merge's addresses have to hold in any case
   } else {
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // ------------------------------------ MMA issuer of chain `warp - kMmaWarp`

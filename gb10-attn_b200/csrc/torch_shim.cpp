@@ -583,6 +583,16 @@ std::tuple<torch::Tensor, torch::Tensor> merge_states(torch::Tensor outs, torch:
   return {out, lse};
 }
 
+// t on `like`'s device with the given type, contiguous; itself if it is so
+// already (the dispatcher's own check of that costs more than these three).
+static torch::Tensor plain(const torch::Tensor& t, const torch::Tensor& like, torch::ScalarType ty) {
+  if (t.device() == like.device() && t.scalar_type() == ty && t.is_contiguous()) return t;
+  return t.to(like.device(), ty).contiguous();
+}
+static torch::Tensor plain_i32(const torch::Tensor& t, const torch::Tensor& like) {
+  return plain(t, like, torch::kInt32);
+}
+
 // The layers' pool tensors as pointer arrays; contiguous and alike.
 struct PoolLayers {
   std::vector<void*> k, v;
@@ -594,6 +604,8 @@ static PoolLayers pool_layers(const std::vector<torch::Tensor>& k_layers,
   const torch::Tensor& k0 = k_layers[0];
   TORCH_CHECK(k0.is_cuda() && k0.dim() == 4, op, ": pool tensors must be CUDA [NB, BS, H, D]");
   PoolLayers p;
+  p.k.reserve(k_layers.size());
+  p.v.reserve(k_layers.size());
   for (size_t l = 0; l < k_layers.size(); ++l) {
     for (const torch::Tensor* t : {&k_layers[l], &v_layers[l]})
       TORCH_CHECK(t->is_contiguous() && t->sizes() == k0.sizes() &&
@@ -608,19 +620,20 @@ static PoolLayers pool_layers(const std::vector<torch::Tensor>& k_layers,
 // Page copies for every layer (pa_copy_blocks): block src_blocks[i] to
 // dst_blocks[i], its first num_rows[i] token rows (an empty tensor: the whole
 // page).  The pool tensors are written in place.
-void copy_blocks(std::vector<torch::Tensor> k_layers, std::vector<torch::Tensor> v_layers,
-                 torch::Tensor src_blocks, torch::Tensor dst_blocks, torch::Tensor num_rows) {
+void copy_blocks(const std::vector<torch::Tensor>& k_layers,
+                 const std::vector<torch::Tensor>& v_layers, const torch::Tensor& src_blocks,
+                 const torch::Tensor& dst_blocks, const torch::Tensor& num_rows) {
   const char* op = "copy_blocks";
   const PoolLayers pl = pool_layers(k_layers, v_layers, op);
   const torch::Tensor& k0 = k_layers[0];
   const c10::cuda::CUDAGuard guard(k0.device());
-  torch::Tensor src = src_blocks.to(k0.device(), torch::kInt32).contiguous();
-  torch::Tensor dst = dst_blocks.to(k0.device(), torch::kInt32).contiguous();
+  torch::Tensor src = plain_i32(src_blocks, k0);
+  torch::Tensor dst = plain_i32(dst_blocks, k0);
   torch::Tensor rows;
   TORCH_CHECK(src.dim() == 1 && dst.sizes() == src.sizes(),
               op, ": src_blocks and dst_blocks must be [n]");
   if (num_rows.defined() && num_rows.numel()) {
-    rows = num_rows.to(k0.device(), torch::kInt32).contiguous();
+    rows = plain_i32(num_rows, k0);
     TORCH_CHECK(rows.sizes() == src.sizes(), op, ": num_rows must be [n] or empty");
   }
   check_status(pa_copy_blocks(pl.k.data(), pl.v.data(), pool_dtype(k0, op), src.data_ptr<int32_t>(),
@@ -637,8 +650,8 @@ torch::Tensor remap_block_tables(torch::Tensor block_tables, torch::Tensor block
   const char* op = "remap_block_tables";
   TORCH_CHECK(block_tables.is_cuda(), "block_tables must be on CUDA");
   const c10::cuda::CUDAGuard guard(block_tables.device());
-  torch::Tensor bt = block_tables.to(torch::kInt32).contiguous();
-  torch::Tensor map = block_map.to(bt.device(), torch::kInt32).contiguous();
+  torch::Tensor bt = plain_i32(block_tables, block_tables);
+  torch::Tensor map = plain_i32(block_map, bt);
   TORCH_CHECK(map.dim() == 1, op, ": block_map must be [num_blocks]");
   torch::Tensor out = torch::empty_like(bt);
   check_status(pa_remap_block_tables(out.data_ptr<int32_t>(), bt.data_ptr<int32_t>(),
@@ -687,13 +700,13 @@ torch::Tensor qk_norm_rope_append(torch::Tensor q, torch::Tensor k, torch::Tenso
   torch::Tensor qs = q.stride(2) == 1 ? q : q.contiguous();
   torch::Tensor ks = k.stride(2) == 1 ? k : k.contiguous();
   torch::Tensor vs = v.stride(2) == 1 ? v : v.contiguous();
-  torch::Tensor cs = cos_sin.to(q.device()).contiguous();
-  torch::Tensor pos = positions.to(q.device(), torch::kInt32).contiguous();
-  torch::Tensor bt = block_tables.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor cs = plain(cos_sin, q, torch::kFloat);
+  torch::Tensor pos = plain_i32(positions, q);
+  torch::Tensor bt = plain_i32(block_tables, q);
   TORCH_CHECK(pos.numel() == T && bt.dim() == 2, op, ": positions [T] and block_tables [B, MB] needed");
   torch::Tensor ids;
   if (seq_ids.defined() && seq_ids.numel()) {
-    ids = seq_ids.to(q.device(), torch::kInt32).contiguous();
+    ids = plain_i32(seq_ids, q);
     TORCH_CHECK(ids.numel() == T, op, ": seq_ids must be [T] or empty");
   } else {
     TORCH_CHECK(T <= bt.size(0), op, ": without seq_ids, block_tables needs a row per token");
@@ -703,7 +716,7 @@ torch::Tensor qk_norm_rope_append(torch::Tensor q, torch::Tensor k, torch::Tenso
     const torch::Tensor& src = i ? k_weight : q_weight;
     if (!src.defined() || !src.numel()) continue;
     TORCH_CHECK(src.numel() == D, op, ": weights must be [D] or empty");
-    w[i] = src.to(q.device()).contiguous();
+    w[i] = plain(src, q, src.scalar_type());
   }
   // one type for both weights: q's, or fp32
   bool w_f32 = false;
@@ -714,7 +727,7 @@ torch::Tensor qk_norm_rope_append(torch::Tensor q, torch::Tensor k, torch::Tenso
   for (int i = 0; i < 2; ++i) {
     const torch::Tensor& src = i ? v_scale : k_scale;
     if (!src.defined() || !src.numel()) continue;
-    sc[i] = src.to(q.device(), torch::kFloat).contiguous();
+    sc[i] = plain(src, q, torch::kFloat);
     TORCH_CHECK(sc[i].numel() == HKV, op, ": scales must be [HKV] or empty");
   }
   torch::Tensor out = torch::empty({T, H, D}, q.options());
@@ -752,10 +765,10 @@ std::tuple<torch::Tensor, torch::Tensor> paged_attention_shared(
               op, ": q and the pool must both be float16 or both bfloat16");
   const c10::cuda::CUDAGuard guard(q.device());
   torch::Tensor qc = q.contiguous(), kc = k_cache.contiguous(), vc = v_cache.contiguous();
-  torch::Tensor bt = block_tables.to(q.device(), torch::kInt32).contiguous();
-  torch::Tensor ctx = context_lens.to(q.device(), torch::kInt32).contiguous();
-  torch::Tensor gs = group_starts.to(q.device(), torch::kInt32).contiguous();
-  torch::Tensor pl = prefix_lens.to(q.device(), torch::kInt32).contiguous();
+  torch::Tensor bt = plain_i32(block_tables, q);
+  torch::Tensor ctx = plain_i32(context_lens, q);
+  torch::Tensor gs = plain_i32(group_starts, q);
+  torch::Tensor pl = plain_i32(prefix_lens, q);
   const int64_t B = qc.size(0), H = qc.size(1), D = qc.size(2);
   const int64_t NB = kc.size(0), BS = kc.size(1), HKV = kc.size(2), NG = pl.numel();
   TORCH_CHECK(kc.size(3) == D, op, ": k_cache head_dim must match q");
