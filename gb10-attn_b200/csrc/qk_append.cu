@@ -132,7 +132,9 @@ template <typename P> __device__ __forceinline__ void store4(P* dst, const float
 constexpr int kThreads = 64;
 constexpr int kBatch = 4;  // heads in flight per thread
 
-// One CTA per token.  D / 8 lanes hold a head, eight elements each, so the CTA
+// One CTA per token, or three (q, k, v) while that leaves SMs idle: the loads of
+// the three follow one another otherwise, and a few tokens take that long.
+// D / 8 lanes hold a head, eight elements each, so the CTA
 // works on 1024 / D heads at a time and has four times as many in flight.  A
 // thread keeps its place in the head: the cosines and sines of its four pairs
 // and its eight weights are loaded once for all of its heads.  HBM-bound: a
@@ -150,14 +152,17 @@ __global__ void __launch_bounds__(kThreads) qk_append_kernel(const __grid_consta
   const int64_t pos = p.positions[t];
   S* const q_out = reinterpret_cast<S*>(p.q_out) + t * H * D;
 
+  const int part = gridDim.y == 1 ? -1 : blockIdx.y;  // 0: q, 1: k, 2: v, -1: all
+
   if (pos < 0 || pos >= p.max_pos) {  // a padding token's q is zero, one past the table's is NaN
+    if (part > 0) return;
     if (pos >= 0 && threadIdx.x == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
     const float x = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
     const float2 y[2] = {make_float2(x, x), make_float2(x, x)};
     for (int e = threadIdx.x * 4; e < H * D; e += kThreads * 4) store4<S>(q_out + e, y);
     return;
   }
-  const int64_t row = pool_row(p, t, pos, threadIdx.x == 0);
+  const int64_t row = part == 0 ? -1 : pool_row(p, t, pos, threadIdx.x == 0);
 
   float2 c[2] = {}, s[2] = {};
   if (at.turns) {
@@ -241,10 +246,10 @@ __global__ void __launch_bounds__(kThreads) qk_append_kernel(const __grid_consta
     };
   };
   if (row >= 0) {
-    each(p.v + t * p.v_tok * sizeof(S), p.v_head, HKV, nullptr, false, to_pool(p.v_cache, p.v_scale));
-    each(p.k + t * p.k_tok * sizeof(S), p.k_head, HKV, p.k_weight, true, to_pool(p.k_cache, p.k_scale));
+    if (part != 1) each(p.v + t * p.v_tok * sizeof(S), p.v_head, HKV, nullptr, false, to_pool(p.v_cache, p.v_scale));
+    if (part != 2) each(p.k + t * p.k_tok * sizeof(S), p.k_head, HKV, p.k_weight, true, to_pool(p.k_cache, p.k_scale));
   }
-  each(p.q + t * p.q_tok * sizeof(S), p.q_head, H, p.q_weight, true, [&](int h, float2 (&y)[4]) {
+  if (part <= 0) each(p.q + t * p.q_tok * sizeof(S), p.q_head, H, p.q_weight, true, [&](int h, float2 (&y)[4]) {
     store4<S>(q_out + h * D + at.a, y);
     store4<S>(q_out + h * D + at.b, y + 2);
   });
@@ -336,7 +341,10 @@ static int launch_typed(const Params& p, cudaStream_t s) {
                     aligned16(p.k_cache) && aligned16(p.v_cache) && aligned16(p.q_weight) &&
                     aligned16(p.k_weight) && aligned16(p.cos_sin) && p.R % 8 == 0;
   if (wide && p.T <= 0x7fffffff && p.H * D <= 0x7fffffff) {
-    qk_append_kernel<S, P><<<(unsigned)p.T, kThreads, 0, s>>>(p);
+    int sms = 0;
+    if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
+    const unsigned parts = p.T <= 4 * sms ? 3 : 1;
+    qk_append_kernel<S, P><<<dim3((unsigned)p.T, parts), kThreads, 0, s>>>(p);
   } else {
     const int64_t ctas = (p.T * heads + kThreads / 32 - 1) / (kThreads / 32);
     if (ctas > 0x7fffffff) return PA_ERR_TOO_LARGE;
