@@ -52,20 +52,24 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) warps_kernel(const __gr
 }
 
 // ---------------------------------------------------------------------------
-// merge: one warp per output row, pieces in a fixed order
+// merge: W warps per output row, each a run of its pieces, all in a fixed order
 // ---------------------------------------------------------------------------
 
-template <typename T, int D>
+template <typename T, int D, int W>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params p) {
   constexpr int E = D / 32;
+  __shared__ float part[W > 1 ? W : 1][W > 1 ? D : 1];
+  __shared__ float2 part_ml[W > 1 ? W : 1];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
   if (row >= p.B * p.H) return;
   const Pieces at = load_plan(p.pieces + row);
   const int32_t own_rows = min(p.G, ROWS), n_pre = at.n_pre, n_own = at.n_own;
-  const int n = n_pre + n_own;
+  const int all = n_pre + n_own, first = W > 1 ? all * warp / W : 0;
+  const int n = W > 1 ? all * (warp + 1) / W - first : all;
   auto piece = [&](int c) -> int64_t {
+    c += first;
     return c < n_pre ? at.pre0 + (int64_t)c * at.pre_step : at.own0 + (int64_t)(c - n_pre) * own_rows;
   };
   // 32 pieces at a time, lane c with the maximum and sum of piece c; then their
@@ -120,6 +124,30 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(in ? wc : 0.f, in ? x[k][e] : 0.f, acc[e]);
       }
+    }
+  }
+  if constexpr (W > 1) {
+    static_assert(W == 8, "the CTA's warps");
+    if (lane == 0) part_ml[warp] = make_float2(M, L);
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[warp][(e / V * 32 + lane) * V + e % V] = acc[e];
+    __syncthreads();
+    if (warp) return;
+    M = lane < W ? part_ml[lane].x : -INFINITY;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    const float base = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float2 ml = part_ml[w];
+      const float f = fast_exp2(ml.x - base);
+      L = fmaf(f, ml.y, L);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, part[w][(e / V * 32 + lane) * V + e % V], acc[e]);
     }
   }
   // no key, or only scores of -inf: L = 0, so out is NaN and lse -inf
@@ -215,7 +243,11 @@ static int launch_typed(const Params& p, int sms, cudaStream_t s) {
     e = launch(kern, sms, C::WARPS * 32, C::SMEM, s, p, p.planned);
     if (e != cudaSuccess) return cuda_status(e);
   }
-  return cuda_status(launch(merge_kernel<T, D>, (p.B * p.H + 7) / 8, 256, 0, s, p, true));
+  // Eight warps a row while one CTA each fits the GPU at once (few rows have
+  // many pieces: with one warp, a sequence of 20k alone took 46 us, 30 of them
+  // here), else one
+  if (p.B * p.H <= 8 * sms) return cuda_status(launch(merge_kernel<T, D, 8>, p.B * p.H, 256, 0, s, p, true));
+  return cuda_status(launch(merge_kernel<T, D, 1>, (p.B * p.H + 7) / 8, 256, 0, s, p, true));
 }
 
 template <typename T>
