@@ -139,15 +139,22 @@ constexpr int kBatch = 4;  // heads in flight per thread
 // thread keeps its place in the head: the cosines and sines of its four pairs
 // and its eight weights are loaded once for all of its heads.  HBM-bound: a
 // token's q, k and v are read once and written once.
-template <typename S, typename P>
+//   TOKENS 2: a warp per token, for tokens whose query heads (H D <= 1024) fill
+// no more than the four heads that a warp's lanes have in flight; twice the
+// tokens are under way then (17873 tokens of 8 + 2 heads of 128 in bf16: 40 us
+// with 1, 29 with 2).
+template <typename S, typename P, int TOKENS>
 __global__ void __launch_bounds__(kThreads) qk_append_kernel(const __grid_constant__ Params p) {
   using R4 = typename Raw4<S>::T;
+  constexpr int kTeam = kThreads / TOKENS;  // threads of a token
+  const int tid = threadIdx.x % kTeam;
   const int lph = 1 << p.lph_shift;  // lanes per head, D / 8
-  const int sub = threadIdx.x & (lph - 1), grp = threadIdx.x >> p.lph_shift;
-  const int groups = kThreads >> p.lph_shift;
-  const int warp_grp = (threadIdx.x & ~31) >> p.lph_shift;  // the warp's first group
+  const int sub = tid & (lph - 1), grp = tid >> p.lph_shift;
+  const int groups = kTeam >> p.lph_shift;
+  const int warp_grp = (tid & ~31) >> p.lph_shift;  // the warp's first group
   const int D = lph * 8, H = (int)p.H, HKV = (int)p.HKV;
-  const int64_t t = blockIdx.x;
+  const int64_t t = (int64_t)blockIdx.x * TOKENS + threadIdx.x / kTeam;
+  if (TOKENS > 1 && t >= p.T) return;
   const Place at = place(p, sub);
   const int64_t pos = p.positions[t];
   S* const q_out = reinterpret_cast<S*>(p.q_out) + t * H * D;
@@ -156,13 +163,13 @@ __global__ void __launch_bounds__(kThreads) qk_append_kernel(const __grid_consta
 
   if (pos < 0 || pos >= p.max_pos) {  // a padding token's q is zero, one past the table's is NaN
     if (part > 0) return;
-    if (pos >= 0 && threadIdx.x == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
+    if (pos >= 0 && tid == 0) report(p.dev_status, PA_DEVERR_CONTEXT);
     const float x = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
     const float2 y[2] = {make_float2(x, x), make_float2(x, x)};
-    for (int e = threadIdx.x * 4; e < H * D; e += kThreads * 4) store4<S>(q_out + e, y);
+    for (int e = tid * 4; e < H * D; e += kTeam * 4) store4<S>(q_out + e, y);
     return;
   }
-  const int64_t row = part == 0 ? -1 : pool_row(p, t, pos, threadIdx.x == 0);
+  const int64_t row = part == 0 ? -1 : pool_row(p, t, pos, tid == 0);
 
   float2 c[2] = {}, s[2] = {};
   if (at.turns) {
@@ -343,8 +350,12 @@ static int launch_typed(const Params& p, cudaStream_t s) {
   if (wide && p.T <= 0x7fffffff && p.H * D <= 0x7fffffff) {
     int sms = 0;
     if (device_sm_count(&sms) != PA_OK) return PA_ERR_NO_DEVICE;
-    const unsigned parts = p.T <= 4 * sms ? 3 : 1;
-    qk_append_kernel<S, P><<<dim3((unsigned)p.T, parts), kThreads, 0, s>>>(p);
+    if (p.T <= 4 * sms)
+      qk_append_kernel<S, P, 1><<<dim3((unsigned)p.T, 3), kThreads, 0, s>>>(p);
+    else if (p.H * D <= 1024)
+      qk_append_kernel<S, P, 2><<<(unsigned)((p.T + 1) / 2), kThreads, 0, s>>>(p);
+    else
+      qk_append_kernel<S, P, 1><<<(unsigned)p.T, kThreads, 0, s>>>(p);
   } else {
     const int64_t ctas = (p.T * heads + kThreads / 32 - 1) / (kThreads / 32);
     if (ctas > 0x7fffffff) return PA_ERR_TOO_LARGE;

@@ -141,7 +141,10 @@ __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
   return kScanBytes + (2 * B + 3 * (NG + 1)) * 4;
 }
 
-constexpr int kMinTiles = 4;    // 16-key tiles per warp when there are few
+// 16-key tiles per warp when there are few: 2, 3, 4 give 12.8, 13.3, 14.3 us for
+// four samples of 512 tokens, 29.9, 23.7, 22.0 for one sequence of 20k (its
+// pieces are more to merge).
+constexpr int kMinTiles = 3;
 constexpr int kTcMinTiles = 6;  // 64-key tiles per CTA below which the warps do all
 // Tiles that a unit costs beside its own (swept: 1, 2, 4 of 16 keys and 2, 5, 8,
 // 14 of 64 keys give 76-82 us for 128 sequences on 8k, 56-60 for seven prompts,

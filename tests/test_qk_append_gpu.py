@@ -219,3 +219,20 @@ def test_shim_refusals():
                      ({"q": q[..., :48], "k": k[..., :48], "v": v[..., :48]}, "head_dim")):
         with pytest.raises(RuntimeError, match=text):
             call(**kw)
+
+
+@pytest.mark.parametrize("H,HKV,D,lens", [(8, 1, 128, [700, 1]), (16, 2, 64, [601, 60]), (32, 8, 128, [640]),
+                                          (4, 4, 256, [593, 7]), (30, 3, 32, [900])])
+def test_many_tokens(H, HKV, D, lens):
+    """Enough tokens that a CTA takes whole tokens, one or two: padding among them, an odd count."""
+    q, k, v, pos, seq, bt, kc, vc, cs, w = case(13, lens, [9, 40][:len(lens)], H, HKV, D, D, torch.bfloat16,
+                                                torch.bfloat16)
+    w = [x.to(torch.bfloat16) for x in w]
+    pos[5] = -1
+    out = ops.qk_norm_rope_append(q, k, v, w[0], w[1], 1e-6, cs, False, pos, seq, kc, vc, bt, NONE, NONE)
+    live = pos >= 0
+    rows = cs[pos[live].long()].double()
+    near(out[live], formula(q[live].to(F64), w[0].to(F64), 1e-6, rows, D, False), torch.bfloat16)
+    at = flat(bt, seq[live], pos[live], 16)
+    near(kc.view(-1, HKV, D)[at], formula(k[live].to(F64), w[1].to(F64), 1e-6, rows, D, False), torch.bfloat16)
+    assert torch.equal(vc.view(-1, HKV, D)[at], v[live]) and bool((out[5] == 0).all())
