@@ -4,14 +4,23 @@
 // cores with S, P and O in tensor memory, then the rest, a warp at a time
 // (shared.cuh).
 //
-// A CTA (one per SM) takes its run of 128-key tiles and walks the units that it
+// A CTA (one per SM) takes its run of 64-key tiles and walks the units that it
 // crosses: the members' query heads of one KV head are the rows of S = Q K^T and
 // O = P V.  Two softmax warpgroups run two chains: rows 0-127 and 128-255 of a
 // unit, or, in a unit of at most 128 rows, the same rows on every other tile,
 // so that one chain's exponentials overlap the other's products.
-// Thread = row = TMEM lane: it reads its 64 scores of a tile, keeps the
-// row's reference maximum and sum in fp32 and writes P over S.  Two warps feed K and V by tiled
-// TMA, 16 rows at a time through the pages; one thread per chain issues its MMAs.
+// Thread = row = TMEM lane: it reads its 64 scores of a tile, keeps the row's
+// reference maximum and sum in fp32 and writes P over S.  Two warps feed K and V
+// by tiled TMA, 16 rows at a time through the pages; one thread per chain issues
+// its MMAs.
+//   Bound by the softmax warps and the MMAs together, then (the sequences' own
+// tokens) by HBM.  256 sequences of 32 / 8 heads of 128 behind 32768 tokens, with
+// 256 to 1024 of their own, take 260 us: the prefix part 130 (1.05 PFLOP/s of S
+// and P V, 63 % of the bf16 burst rate, 76 % of the sustained one), the own tokens
+// 105 (6.4 TB/s).  Tiles of 64 keys, not 128: two S of each chain then fit the
+// tensor memory beside both O, and S of the next tile is computed while a chain
+// works on this one (an MMA of N = 64 takes 48 cycles, of N = 128 64, but the
+// pipe waits less).
 //   Precision: one 16-bit product each for S (Q and K as they are, products
 // exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be; the
 // sum l is of the unrounded weights).  The scale is applied to S in fp32.
@@ -78,7 +87,8 @@ __device__ __forceinline__ void store32(float* dst, const uint32_t* v) {
 }
 
 // One lane of the warp, in a form that the compiler knows for a single thread's:
-// its branch keeps the operands of the MMAs in uniform registers.
+// its branch keeps the operands of the MMAs in uniform registers (32 cycles to
+// issue one; 47 behind a test of the lane's number).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;}" : "=r"(p));
