@@ -12,8 +12,8 @@
 // Two launches, the second a programmatic dependent of the first: the attention
 // and the merge of its partials.  Every CTA of the first makes the same plan in
 // shared memory (the groups' usable prefixes, running counts of the work) and
-// takes an equal run of the work; only for many sequences the plan is a launch
-// of its own.
+// takes an equal run of one kind of work; only for many sequences the plan is a
+// launch of its own.
 #include <algorithm>
 #include <mutex>
 #include <vector>
@@ -47,8 +47,9 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) warps_kernel(const __gr
   pdl_trigger();
   const Plan plan = take_plan(p, smem);
   // consecutive workers sit on different SMs
-  warp_work<T, D, Cfg<D>::STAGES>(p, plan, load_plan(plan.totals), smem_u32(smem) + warp * Cfg<D>::RING,
-                                  (int64_t)warp * gridDim.x + blockIdx.x);
+  const int64_t worker = (int64_t)warp * gridDim.x + blockIdx.x;
+  warp_work<T, D, Cfg<D>::STAGES>(p, plan, load_plan(plan.totals), smem_u32(smem) + warp * Cfg<D>::RING, worker,
+                                  worker);
 }
 
 // ---------------------------------------------------------------------------

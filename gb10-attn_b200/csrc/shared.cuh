@@ -30,7 +30,7 @@ constexpr int TC_ROWS = 256;
 // that meet a unit's start have less to read.  A piece of these alone is empty.
 //   The prefixes of groups with many rows are done in tensor memory
 // (shared_tc.cu), with tiles, units and workers (CTAs) of their own, numbered
-// the same way.
+// the same way.  Some CTAs do these then and the others' warps the rest.
 struct alignas(16) Group {
   long long tile0[2];           // first tile: of the warps' work, of the tensor memory's
   int32_t b0, n, table, prefix; // members b0 .. b0 + n - 1; table row that serves; tokens shared
@@ -43,6 +43,7 @@ struct alignas(16) Seq {
 struct alignas(16) Totals {
   int64_t prefix_tiles, tiles, workers;  // the warps' work
   int64_t tc_tiles, tc_workers;          // the tensor memory's
+  int64_t own_cta0, pad;                 // first CTA whose warps take work
 };
 
 // Where the partials of an output row are: n_pre pieces of its prefix unit,
@@ -136,7 +137,7 @@ __device__ __forceinline__ Plan plan_at(const Params& p, int64_t copy) {
 // Sequences and groups up to which every CTA makes the plan itself, in shared
 // memory, if its counts fit 32 bits: one launch less, which small calls notice.
 constexpr int kPlanMax = 1024;
-constexpr int64_t kScanBytes = 2 * 32 * 40 + 16;  // the scans' sums, a counter
+constexpr int64_t kScanBytes = 2 * 32 * 40 + 16;  // the scans' sums, two counters
 __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
   return kScanBytes + (2 * B + 3 * (NG + 1)) * 4;
 }
@@ -151,6 +152,13 @@ constexpr int kTcMinTiles = 6;  // 64-key tiles per CTA below which the warps do
 // each best at another; these are within 3 % of the best of both).
 constexpr int kUnitCost = 2;
 constexpr int kTcUnitCost = 6;
+
+// What a warps' tile and a tensor-memory tile of one chain's rows cost an SM,
+// in percent of a tensor-memory tile of both chains (0.15 and 1.2 us).  Swept: 11,
+// 12, 13 with 75 to 85 give 260, 268, 245 us for 256 sequences on 32k (too few
+// CTAs for the own tokens are dear there), 63, 63, 65 for 128 on 8k, 50 for seven
+// prompts with any of them.
+constexpr double kTileCost = 13, kTcSmallCost = 85;
 
 // Tiles that a unit of `keys` keys counts as.
 __host__ __device__ __forceinline__ int32_t unit_tiles(int32_t keys) { return keys ? cdiv(keys, KT) + kUnitCost : 0; }
@@ -198,12 +206,14 @@ template <typename I>
 __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void* scratch, bool tell) {
   using S = Sums<I, 5>;
   auto sums = static_cast<S(*)[32]>(scratch);
-  unsigned long long& tc_work = *reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + 2 * 32 * 40);
+  // the tensor memory's tiles if it takes what it may, and those of them in
+  // units of one chain's rows
+  auto tc_work = reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + 2 * 32 * 40);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int32_t B = (int32_t)p.B, NG = (int32_t)p.NG, HKV = (int32_t)p.HKV, G = p.G;
   const int32_t max_ctx = (int32_t)min(p.MB * p.BS, (int64_t)0x7fffff00);
   int32_t *ctx = reinterpret_cast<int32_t*>(static_cast<char*>(scratch) + kScanBytes), *grp = ctx + B, *gs = grp + B, *pre = gs + NG + 1, *lead = pre + NG + 1;
-  if (tid == 0) tc_work = 0;
+  if (tid == 0) tc_work[0] = tc_work[1] = 0;
   int far = 0;
   for (int32_t b = tid; b < B; b += threads) {
     const int32_t c = p.context_lens[b];
@@ -238,12 +248,16 @@ __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void
       const int32_t prefix = live > 1 ? max(0, min(pre[g], least)) : 0;
       pre[g] = prefix;
       lead[g] = first;
-      if (p.tc_rows && (e - a) * G >= p.tc_rows)
-        atomicAdd(&tc_work, (unsigned long long)HKV * cdiv((e - a) * G, TC_ROWS) * tc_unit_tiles(prefix));
+      const int32_t rows = (e - a) * G;
+      if (p.tc_rows && rows >= p.tc_rows) {
+        const unsigned long long n = (unsigned long long)HKV * tc_unit_tiles(prefix);
+        atomicAdd(&tc_work[0], n * cdiv(rows, TC_ROWS));
+        if ((rows - 1) % TC_ROWS < TC_ROWS / 2) atomicAdd(&tc_work[1], n);
+      }
     }
   }
   __syncthreads();
-  const bool use_tc = p.tc_rows && tc_work >= (unsigned long long)kTcMinTiles * p.tc_ctas;
+  const bool use_tc = p.tc_rows && tc_work[0] >= (unsigned long long)kTcMinTiles * p.tc_ctas;
   // running counts: the groups' tiles and units (the warps', the tensor
   // memory's), the sequences' tiles
   S base = {};
@@ -270,8 +284,21 @@ __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void
   }
   if (tid == 0) {
     const int64_t tiles = (int64_t)base.v[0] + base.v[4], tc_tiles = base.v[1];
-    *out.totals = Totals{base.v[0], tiles, min((int64_t)p.warps, max((tiles + kMinTiles - 1) / kMinTiles, (int64_t)1)),
-                         tc_tiles, min((int64_t)p.tc_ctas, max(tc_tiles, (int64_t)1))};
+    // The CTAs that take the warps' work: with tensor-memory work beside it as
+    // many as their part of the cost, so that both end together.  (All CTAs for
+    // one and then for the other leave HBM idle first and the tensor cores next:
+    // 256 sequences on 32k 260 us, so 245, 128 on 8k 74 and 65, seven prompts 57 and
+    // 50.)
+    int64_t own0 = 0, own_ctas = p.tc_ctas, tc_ctas = p.tc_ctas;
+    if (tc_tiles && tiles && tc_ctas > 1) {
+      const double own = (double)kTileCost * (double)tiles;
+      const double tc = 100. * (double)tc_work[0] - (100. - kTcSmallCost) * (double)tc_work[1];
+      own_ctas = min(max((int64_t)(own / (own + tc) * p.tc_ctas + 0.5), (int64_t)1), tc_ctas - 1);
+      tc_ctas -= own_ctas;
+      own0 = tc_ctas;
+    }
+    const int64_t warps = min((int64_t)p.warps / p.tc_ctas * own_ctas, max((tiles + kMinTiles - 1) / kMinTiles, (int64_t)1));
+    *out.totals = Totals{base.v[0], tiles, warps, tc_tiles, min(tc_ctas, max(tc_tiles, (int64_t)1)), own0, 0};
   }
   __syncthreads();
 }
@@ -464,12 +491,13 @@ __device__ __forceinline__ void locate_rows(const Params& p, const Plan& plan, c
 // to the pool's type for the second product (by 2^-9 or 2^-12 of a weight at most
 // and averaged over the keys: at the level of the output's own rounding); the
 // sum l is of the unrounded weights.
-//   HBM-bound on long runs: 256 sequences' own 671 MB of 8 KV heads of 128 in
-// 105 us (6.4 TB/s).  Bound by latency, some three stages an item, where units have
-// a tile or two: 181 sequences of 32 / 32 heads, 85 MB in all, take 62 us.
+//   HBM-bound on long runs on all SMs: 256 sequences' own 671 MB of 8 KV heads of 128
+// in 105 us (6.4 TB/s).  On fewer of them bound by the latency of its instructions,
+// 0.15 us a tile and SM, and some four such an item where units have a tile or two:
+// 181 sequences of 32 / 32 heads, 85 MB in all, take 57 us.
 template <typename T, int D, int NST>
 __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, const Totals& tot, uint32_t ring,
-                                          int64_t worker) {
+                                          int64_t worker, int64_t index) {
   constexpr int CH = D / 8;  // 16-byte chunks per row
   constexpr uint32_t STAGE = stage_bytes(D), NONE = 0xffffffffu;
   const int lane = threadIdx.x & 31;
@@ -562,7 +590,7 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
   };
 
   // While the first bytes are on their way
-  locate_rows(p, plan, tot, worker);
+  locate_rows(p, plan, tot, index);
 
   // ---- the products' side
   const int mi = lane >> 3, mr = lane & 7;  // matrix and row that this lane addresses

@@ -1,10 +1,10 @@
 // shared_tc.cu -- the attention launch of the shared-prefix decode for pools
 // that tiled TMA can load (whole 16-row groups inside a page, head_dim 64 or
 // 128): first the prefixes shared by many query rows, on the sm_100a tensor
-// cores with S, P and O in tensor memory, then the rest, a warp at a time
-// (shared.cuh).
+// cores with S, P and O in tensor memory; beside it, in CTAs of their own, the
+// rest, a warp at a time (shared.cuh).
 //
-// A CTA (one per SM) takes its run of 64-key tiles and walks the units that it
+// A CTA of the first kind takes its run of 64-key tiles and walks the units that it
 // crosses: the members' query heads of one KV head are the rows of S = Q K^T and
 // O = P V.  Two softmax warpgroups run two chains: rows 0-127 and 128-255 of a
 // unit, or, in a unit of at most 128 rows, the same rows on every other tile,
@@ -13,14 +13,15 @@
 // reference maximum and sum in fp32 and writes P over S.  Two warps feed K and V
 // by tiled TMA, 16 rows at a time through the pages; one thread per chain issues
 // its MMAs.
-//   Bound by the softmax warps and the MMAs together, then (the sequences' own
-// tokens) by HBM.  256 sequences of 32 / 8 heads of 128 behind 32768 tokens, with
-// 256 to 1024 of their own, take 260 us: the prefix part 130 (1.05 PFLOP/s of S
-// and P V, 63 % of the bf16 burst rate, 76 % of the sustained one), the own tokens
-// 105 (6.4 TB/s).  Tiles of 64 keys, not 128: two S of each chain then fit the
-// tensor memory beside both O, and S of the next tile is computed while a chain
-// works on this one (an MMA of N = 64 takes 48 cycles, of N = 128 64, but the
-// pipe waits less).
+//   Bound by the softmax warps and the MMAs together (1.2 us a tile of 256 rows: on
+// all SMs 1.05 PFLOP/s of S and P V, 63 % of the bf16 burst rate, 76 % of the
+// sustained one), while the CTAs with the sequences' own tokens are bound by
+// instruction latency (0.15 us a 16-key tile).  256 sequences of 32 / 8 heads of 128
+// behind 32768 tokens, with 256 to 1024 of their own: 245 us, some 88 CTAs with the
+// prefix and 60 with the rest.
+//   Tiles of 64 keys, not 128: two S of each chain then fit the tensor memory
+// beside both O, and S of the next tile is computed while a chain works on this
+// one (an MMA of N = 64 takes 48 cycles, of N = 128 64, but the pipe waits less).
 //   Precision: one 16-bit product each for S (Q and K as they are, products
 // exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be; the
 // sum l is of the unrounded weights).  The scale is applied to S in fp32.
@@ -44,8 +45,8 @@ using prefill::warp_wait_rx;
 constexpr int kMmaWarp = 8, kKWarp = 10, kVWarp = 11;  // (an issuer per chain: 8 and 9)
 constexpr int kTcThreads = 384;
 // 384 threads launched at 168 registers (64512).  After the tensor-memory part
-// the issuing and loading warps give theirs up and the warps' own work takes
-// 240: 256 x 240 + 128 x 24 = 64512.
+// (at once in a CTA that has none of it) the issuing and loading warps give theirs
+// up and the warps' own work takes 240: 256 x 240 + 128 x 24 = 64512.
 constexpr int kWorkRegs = 240, kDoneRegs = 24;
 static_assert(256 * kWorkRegs + 128 * kDoneRegs <= kTcThreads * 168, "register split");
 
@@ -333,11 +334,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     // free for the rings of the warps' own work
     asm volatile("bar.sync 1, 256;" ::: "memory");
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkRegs));
-    const int64_t own = (int64_t)warp * gridDim.x + blockIdx.x;
+    const int64_t index = (int64_t)warp * gridDim.x + blockIdx.x;
+    const int64_t own = blockIdx.x < tot.own_cta0 ? tot.workers
+                                                  : warp * (gridDim.x - tot.own_cta0) + blockIdx.x - tot.own_cta0;
     if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
-      warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, own);
+      warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, own, index);
     else
-      locate_rows(p, plan, tot, own);  // the merge's addresses have to hold in any case
+      locate_rows(p, plan, tot, index);  // the merge's addresses have to hold in any case
   } else {
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // ------------------------------------ MMA issuer of chain `warp - kMmaWarp`
