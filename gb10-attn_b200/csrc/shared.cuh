@@ -287,8 +287,8 @@ __device__ __forceinline__ void make_plan(const Params& p, const Plan& out, void
     // The CTAs that take the warps' work: with tensor-memory work beside it as
     // many as their part of the cost, so that both end together.  (All CTAs for
     // one and then for the other leave HBM idle first and the tensor cores next:
-    // 256 sequences on 32k 260 us, so 245, 128 on 8k 74 and 65, seven prompts 57 and
-    // 50.)
+    // 256 sequences on 32k 260 us, so 245, 128 on 8k 74 and 64, seven prompts 57 and
+    // 51.)
     int64_t own0 = 0, own_ctas = p.tc_ctas, tc_ctas = p.tc_ctas;
     if (tc_tiles && tiles && tc_ctas > 1) {
       const double own = (double)kTileCost * (double)tiles;
@@ -399,8 +399,10 @@ struct Run {
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
+               "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() {
@@ -550,6 +552,11 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
   };
   // Rows of no key or query are zeros: their scores are masked, and no weight
   // of zero meets a NaN of an unwritten row.
+  // They are read once and leave the L2 first, which keeps prefixes that several
+  // units read (128 sequences on 8k 64 -> 61 us, 100 of 24 / 8 heads on 4k 55 -> 52,
+  // 14 on 15k 27 -> 25.5; 256 on 32k 238 -> 246).
+  uint64_t once;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
   auto fill = [&](uint32_t st, int kind, uint32_t row) {
     if (kind) {
       const char* a = static_cast<const char*>(kind == 1 ? p.q : p.k);
@@ -559,9 +566,9 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
         const uint32_t pr = __shfl_sync(0xffffffffu, row, r);
         const int bytes = pr == NONE ? 0 : 16;
         const int64_t off = bytes ? ((int64_t)pr * CH + c) * 16 : 0;
-        cp_async16(ring + st + chunk_at(r, c), a + off, bytes);
+        cp_async16(ring + st + chunk_at(r, c), a + off, bytes, once);
         if (kind == 2)
-          cp_async16(ring + st + KT * D * 2 + chunk_at(r, c), static_cast<const char*>(p.v) + off, bytes);
+          cp_async16(ring + st + KT * D * 2 + chunk_at(r, c), static_cast<const char*>(p.v) + off, bytes, once);
       }
     }
     cp_async_commit();

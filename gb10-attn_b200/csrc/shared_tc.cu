@@ -17,7 +17,7 @@
 // all SMs 1.05 PFLOP/s of S and P V, 63 % of the bf16 burst rate, 76 % of the
 // sustained one), while the CTAs with the sequences' own tokens are bound by
 // instruction latency (0.15 us a 16-key tile).  256 sequences of 32 / 8 heads of 128
-// behind 32768 tokens, with 256 to 1024 of their own: 245 us, some 88 CTAs with the
+// behind 32768 tokens, with 256 to 1024 of their own: 246 us, some 88 CTAs with the
 // prefix and 60 with the rest.
 //   Tiles of 64 keys, not 128: two S of each chain then fit the tensor memory
 // beside both O, and S of the next tile is computed while a chain works on this
