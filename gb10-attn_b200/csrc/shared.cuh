@@ -552,7 +552,7 @@ __device__ __forceinline__ void warp_work(const Params& p, const Plan& plan, con
   };
   // Rows of no key or query are zeros: their scores are masked, and no weight
   // of zero meets a NaN of an unwritten row.
-  // They are read once and leave the L2 first, which keeps prefixes that several
+  // Most are read once: all leave the L2 first, which keeps prefixes that several
   // units read (128 sequences on 8k 64 -> 61 us, 100 of 24 / 8 heads on 4k 55 -> 52,
   // 14 on 15k 27 -> 25.5; 256 on 32k 238 -> 246).
   uint64_t once;
