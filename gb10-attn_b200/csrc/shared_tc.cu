@@ -226,7 +226,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       const bool by_keys = im.rows <= 128;
       const int row = by_keys ? r : 128 * c + r;  // of the unit
       const int tiles = by_keys ? (im.n - c + 1) / 2 : im.n;
-      if (im.n > 0) {
+      // (Q is handed over only with a tile: an item that has none for this chain,
+      // one of a single tile by keys, ends without a wait on its issuer, who may not
+      // fall behind by the two phases that a parity cannot tell apart)
+      if (tiles > 0) {
         unsigned char* qd = smem + c * C::QTILE;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k)
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       const uint64_t vd = tc::smem_desc_sw128(smem_u32(smem) + C::OFF_V, TC_KT * 128, 1024);
       const uint32_t scol = tmem + C::COL_S + 128 * c, ocol = tmem + C::COL_O + 128 * c;
       uint32_t kn = 0, kp = 0, vn = 0, vp = 0;  // stage and phase of the coming K and V tile
-      uint32_t items = 0, ns = 0, np = 0;       // items; S and P V of this chain
+      uint32_t items = 0, ns = 0, np = 0;       // items with tiles, S and P V of this chain
       bool ok = true;
       if (elect_one()) while (walk.next(p, worker, im)) {
         if (!ok || im.n == 0) continue;
@@ -389,7 +392,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           }
           return true;
         };
-        ok = mbar_wait(&q_ready[c], items & 1, abort_s) && start(false) && start(false);
+        const bool any = !by_keys || im.n > c;
+        ok = (!any || mbar_wait(&q_ready[c], items & 1, abort_s)) && start(false) && start(false);
         while (tv < im.n && ok) {
           if (!mbar_wait(&v_full[vn], vp, abort_s)) { ok = false; break; }
           const bool mine = own(tv++);
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           if (mine) ok = start(true);
         }
         if (!ok) report(p.dev_status, PA_DEVERR_TIMEOUT);
-        ++items;
+        items += any;
       }
     } else if (warp == kKWarp || warp == kVWarp) {
       // ---------------------------------------------------- K and V producers
