@@ -175,6 +175,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 // Rows of a group from which its prefix may go to the tensor memory.
 constexpr int kTcRows = 33;
 
+constexpr int64_t kAlign = 256;  // of the workspace's parts
+
 struct Layout {
   bool tc, planned;
   int64_t warps, plan_bytes, group_off, seq_off, scratch_off, own_row0, tc_row0;
@@ -188,7 +190,9 @@ static int warps_per_cta(int64_t D) {
 // Slots for partials: unit + worker < units + workers, for prefixes with ROWS
 // rows each, for sequences' own units with min(G, ROWS), for the tensor
 // memory's with TC_ROWS.  `tc`: whether this launch has that part (a size query,
-// which does not know the pool, assumes the larger).
+// which does not know the pool, assumes the larger).  Offsets are multiples of 256
+// from the workspace's first address that is one (partials are stored 32 bytes at
+// a time); `total` has room for the bytes before it.
 static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int sms, bool tc, int64_t max_ctx,
                   Layout* y) {
   const int64_t G = H / HKV;
@@ -201,18 +205,18 @@ static int layout(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int 
   int64_t rows = y->tc_row0;
   if (y->tc) rows += (HKV * (B * G / TC_ROWS + std::min<int64_t>(NG, B * G / kTcRows)) + sms) * TC_ROWS;
   if (rows >= (int64_t(1) << 31) || B * H >= (int64_t(1) << 31)) return PA_ERR_TOO_LARGE;
-  auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  auto up = [](int64_t x) { return (x + kAlign - 1) & ~(kAlign - 1); };
   // tiles of every unit if all had the longest context
   const double most_tiles = (double)(pre_units + own_units) * ((double)max_ctx / KT + 1 + kTcUnitCost);
   y->planned = B > kPlanMax || NG > kPlanMax || most_tiles >= 2147483647.0;
-  y->group_off = 256;
+  y->group_off = kAlign;
   y->seq_off = y->group_off + up(NG * (int64_t)sizeof(Group));
   y->scratch_off = y->seq_off + up(B * (int64_t)sizeof(Seq));
   y->plan_bytes = y->scratch_off + (y->planned ? up(plan_scratch(B, NG)) : 0);
   y->pieces = (size_t)(y->plan_bytes * (y->planned ? 1 : sms));
   y->ml = y->pieces + (size_t)up(B * H * (int64_t)sizeof(Pieces));
   y->o = y->ml + (size_t)up(rows * (int64_t)sizeof(float2));
-  y->total = y->o + (size_t)up(rows * D * (int64_t)sizeof(float));
+  y->total = y->o + (size_t)up(rows * D * (int64_t)sizeof(float)) + kAlign - 16;
   return PA_OK;
 }
 
@@ -328,7 +332,8 @@ extern "C" int pa_paged_attention_shared(
   if (st) return st;
   if (!workspace || workspace_bytes < y.total) return PA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PA_ERR_ALIGNMENT;
-  char* ws = static_cast<char*>(workspace);
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + shared::kAlign - 1) &
+                                     ~(uintptr_t)(shared::kAlign - 1));
   shared::Params p = {};
   p.out = out;
   p.lse = lse;

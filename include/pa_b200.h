@@ -515,7 +515,8 @@ PA_API int pa_qk_norm_rope_append(
     int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t max_blocks,
     int32_t* dev_status, void* stream);
 
-/* Bytes of scratch pa_paged_attention_shared needs for these sizes. */
+/* Bytes of scratch pa_paged_attention_shared needs for these sizes; the
+ * scratch has to start on a 16-byte boundary, as q, out and the pools. */
 PA_API int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_heads,
                                     int64_t num_kv_heads, int64_t head_dim, int kv_dtype,
                                     size_t* bytes);

@@ -24,26 +24,30 @@ def in_tensor_memory(groups, G, HKV):
     return tiles >= 6 * torch.cuda.get_device_properties(0).multi_processor_count
 
 
-def call(q, kc, vc, bt, ctx, gs, pl, scale):
-    """Through the C ABI: (out, lse, the device's status)."""
+def call(q, kc, vc, bt, ctx, gs, pl, scale, offset=0):
+    """Through the C ABI: (out, lse, the device's status).  The workspace starts `offset` bytes past a 512-byte
+    boundary; what lies around it has to stay."""
     B, H, D = q.shape
     NB, BS, HKV, _ = kc.shape
     NG = pl.numel()
     n = ctypes.c_size_t()
     _lib.check("ws", _lib.call("pa_shared_workspace_size", B, NG, H, HKV, D, DT[q.dtype], ctypes.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    room = torch.full((n.value + 2 * 512,), 0xa5, dtype=torch.uint8, device="cuda")
+    assert room.data_ptr() % 512 == 0
+    ws = room[offset:offset + n.value]
     out, lse = torch.empty_like(q), torch.empty((B, H), device="cuda")
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     _lib.check("shared", _lib.call("pa_paged_attention_shared", ptr(out), ptr(lse), ptr(q), DT[q.dtype], ptr(kc),
                                    ptr(vc), DT[q.dtype], ptr(bt), ptr(ctx), ptr(gs), ptr(pl), B, NG, H, HKV, D, BS, NB,
                                    bt.shape[1], scale, ptr(ws), n.value, ptr(status), stream()))
+    assert bool((room[:offset] == 0xa5).all()) and bool((room[offset + n.value:] == 0xa5).all())
     return out, lse, int(status)
 
 
-def check(args, scale=None, status=0):
+def check(args, scale=None, status=0, **kw):
     q, kc, vc, bt, ctx, gs, pl = args
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    out, lse, got = call(*args, scale)
+    out, lse, got = call(*args, scale, **kw)
     assert got == status
     near(out, lse, *formula(q, kc, vc, bt, ctx, scale), q.dtype)
 
@@ -63,3 +67,11 @@ def equal_groups(seed, groups, members, prefixes, tail, H, HKV, D, dtype, BS=16)
 def test_many_groups_of_short_prefixes(groups, members, H, HKV, prefixes, D, dtype, tail):
     """Units of one tile and of few in long rows: with one tile only one of the two chains has work."""
     check(equal_groups(D + tail, groups, members, prefixes, tail, H, HKV, D, dtype))
+
+
+@pytest.mark.parametrize("offset", [16, 48, 240, 256])
+def test_workspaces_on_any_16_byte_boundary(offset):
+    check(equal_groups(1, 16, 16, (300,), 40, 32, 8, 128, torch.bfloat16), offset=offset)
+    # without the tensor memory, and with the plan as a launch of its own
+    check(make(2, 8, 2, 64, torch.float16, 5, [0, 3], [40], [50, 60, 70]), offset=offset)
+    check(make(3, 4, 2, 64, torch.float16, 16, [0, 1100], [20], [20 + b % 9 for b in range(1100)]), offset=offset)
