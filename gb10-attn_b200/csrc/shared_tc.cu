@@ -101,6 +101,16 @@ struct TcParams {
   Params p;
 };
 
+// Two 16-bit elements times zero: NaN for infinities and NaN, else zero.
+__device__ __forceinline__ uint32_t times_zero(uint32_t w, __half*) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(0.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t times_zero(uint32_t w, __nv_bfloat16*) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(0.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // A unit's part of a CTA's run: rows r0 .. r0 + rows - 1 of the group (at most
 // 256), KV head kvh, tiles j0 .. j0 + n - 1 (n may be 0), keys below `prefix`.
 struct TcItem {
@@ -205,9 +215,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     const int c = warp >> 2, r = (warp & 3) * 32 + lane;  // chain, row of the chain = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ocol = C::COL_O + 128 * c;
-    // S is scaled by |qscale|; a negative scale is in Q's sign bits
-    const float qs = fabsf(p.qscale);
+    // S is scaled by |qscale|; a negative scale is in Q's sign bits, one of zero in
+    // Q too (masked keys are at -inf before the scale, and -inf * 0 is NaN)
+    const bool zero = p.qscale == 0.f;
+    const float qs = zero ? 1.f : fabsf(p.qscale);
     const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;
+    auto signed_q = [&](uint32_t w) { return zero ? times_zero(w, (T*)nullptr) : w ^ flip; };
     uint32_t uses = 0, done = 0;  // tiles, items with tiles of this chain: the phases of its barriers
     bool ok = true;
     // Q of this thread's row of an item (zeros for none: written in any case, so
@@ -234,7 +247,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < D / 8; ++k)
           *reinterpret_cast<uint4*>(qd + sw128_offset(r, 8 * k, 128)) =
-              make_uint4(qr[k].x ^ flip, qr[k].y ^ flip, qr[k].z ^ flip, qr[k].w ^ flip);
+              make_uint4(signed_q(qr[k].x), signed_q(qr[k].y), signed_q(qr[k].z), signed_q(qr[k].w));
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_ready[c]);

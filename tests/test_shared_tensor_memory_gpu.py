@@ -75,3 +75,14 @@ def test_workspaces_on_any_16_byte_boundary(offset):
     # without the tensor memory, and with the plan as a launch of its own
     check(make(2, 8, 2, 64, torch.float16, 5, [0, 3], [40], [50, 60, 70]), offset=offset)
     check(make(3, 4, 2, 64, torch.float16, 16, [0, 1100], [20], [20 + b % 9 for b in range(1100)]), offset=offset)
+
+
+@pytest.mark.parametrize("prefixes", [(40, 64, 1), (300, 100)])
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+def test_scales_of_zero(prefixes, D, dtype):
+    """Every key weighs the same, also by a scale that is zero in 32 bits; NaN and infinities in Q are not lost."""
+    q, kc, vc, bt, ctx, gs, pl = equal_groups(4, 17, 16, prefixes, 20, 32, 8, D, dtype)
+    for scale in (0.0, -0.0, 1e-60):
+        check((q, kc, vc, bt, ctx, gs, pl), scale=scale)
+    q[3, 5, 7], q[20, 31, 0] = float("inf"), float("nan")
+    check((q, kc, vc, bt, ctx, gs, pl), scale=0.0)
