@@ -15,6 +15,7 @@
 // takes an equal run of one kind of work; only for many sequences the plan is a
 // launch of its own.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -177,6 +178,8 @@ constexpr int kTcRows = 33;
 
 constexpr int64_t kAlign = 256;  // of the workspace's parts
 
+static std::atomic<int> g_waits{1};  // pa_set_shared_waits
+
 struct Layout {
   bool tc, planned;
   int64_t warps, plan_bytes, group_off, seq_off, scratch_off, own_row0, tc_row0;
@@ -279,6 +282,8 @@ static int check(int64_t B, int64_t NG, int64_t H, int64_t HKV, int64_t D, int d
 }  // namespace shared
 }  // namespace pa
 
+extern "C" int pa_set_shared_waits(int waits) { return pa::shared::g_waits.exchange(waits != 0); }
+
 extern "C" int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_heads,
                                         int64_t num_kv_heads, int64_t head_dim, int kv_dtype,
                                         size_t* bytes) {
@@ -367,6 +372,7 @@ extern "C" int pa_paged_attention_shared(
   p.tc_row0 = y.tc_row0;
   p.tc_rows = y.tc ? shared::kTcRows : 0;
   p.tc_ctas = sms;
+  p.waits = shared::g_waits.load(std::memory_order_relaxed);
   p.pieces = reinterpret_cast<shared::Pieces*>(ws + y.pieces);
   p.part_ml = reinterpret_cast<float2*>(ws + y.ml);
   p.part_o = reinterpret_cast<float*>(ws + y.o);

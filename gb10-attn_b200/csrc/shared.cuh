@@ -75,6 +75,7 @@ struct Params {
   int64_t tc_row0;  // and of the tensor memory's units
   int32_t tc_rows;  // rows from which a group's prefix goes to the tensor memory (0: none does)
   int32_t tc_ctas;
+  int32_t waits;        // 0: the tensor memory's softmax gives up at its first tile (pa_set_shared_waits)
   int32_t* dev_status;
 };
 

@@ -26,7 +26,8 @@
 // exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be; the
 // sum l is of the unrounded weights).  The scale is applied to S in fp32.
 //   Every wait is bounded; on a timeout the CTA reports PA_DEVERR_TIMEOUT, stops
-// issuing work and still frees its tensor memory.
+// issuing work, makes NaN of the rows in its run, lets its copies and products
+// end and frees its tensor memory.
 #include <algorithm>
 #include <mutex>
 #include <vector>
@@ -63,7 +64,7 @@ template <int D> struct TcCfg {
   static constexpr uint32_t TILE = TC_KT * D * 2;      // K or V of a tile
   static constexpr int NK = D == 128 ? 5 : 12, NV = NK;
   static constexpr uint32_t OFF_K = 2 * QTILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;
-  static constexpr uint32_t N_BARS = 2 * NK + 2 * NV + 14;
+  static constexpr uint32_t N_BARS = 2 * NK + 2 * NV + 16;
   static constexpr uint32_t SMEM = OFF_BAR + N_BARS * 8 + 16 + 1024;  // + alignment slack
   // afterwards the warps' rings, in the same bytes
   static constexpr int STAGES = (int)(OFF_BAR / kTcWarps / stage_bytes(D));
@@ -177,7 +178,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
   uint64_t* o_ready = p_full + 4;    // [2] a chain's P V done
   uint64_t* o_last = o_ready + 2;    // [2] its last P V of an item done
   uint64_t* q_ready = o_last + 2;    // [2] its Q in shared memory
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
+  uint64_t* drained = q_ready + 2;   // [2] every product of a chain done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
   int32_t* abort_s = reinterpret_cast<int32_t*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -193,6 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       mbar_init(&o_ready[c], 1);
       mbar_init(&o_last[c], 1);
       mbar_init(&q_ready[c], 4);
+      mbar_init(&drained[c], 1);
     }
     *abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -222,7 +225,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     const uint32_t flip = p.qscale < 0.f ? 0x80008000u : 0u;
     auto signed_q = [&](uint32_t w) { return zero ? times_zero(w, (T*)nullptr) : w ^ flip; };
     uint32_t uses = 0, done = 0;  // tiles, items with tiles of this chain: the phases of its barriers
-    bool ok = true;
     // Q of this thread's row of an item (zeros for none: written in any case, so
     // that it takes no registers while the tiles are worked on)
     uint4 qr[D / 8];
@@ -234,6 +236,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       for (int k = 0; k < D / 8; ++k) qr[k] = there && row < it.rows ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
     };
     bool more = walk.next(p, worker, im);
+    bool ok = p.waits || !more;  // (a test lets it give up at its first tile)
     load_q(im, more);
     while (more) {
       const bool by_keys = im.rows <= 128;
@@ -345,7 +348,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
         tc::fence_before_sync();
       }
     }
-    if (!ok && lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
+    if (!ok) {
+      // given up: every piece of the run is NaN, done or not, and so are the
+      // output rows that have one
+      tc::tmem_wait_st();
+      if (lane == 0) {
+        atomicExch(abort_s, 1);
+        report(p.dev_status, PA_DEVERR_TIMEOUT);
+      }
+      const float nan = __int_as_float(0x7fc00000);
+      Walk again(p, plan, tot, worker, lane);
+      while (again.next(p, worker, im))
+        if ((im.rows <= 128 ? r : 128 * c + r) < im.rows) p.part_ml[im.prow + 128 * c + r] = make_float2(nan, nan);
+    }
     // Both chains done: every product has been taken, and the shared memory is
     // free for the rings of the warps' own work
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -356,7 +371,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
       warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, own, index);
     else
-      locate_rows(p, plan, tot, index);  // the merge's addresses have to hold in any case
+      locate_rows(p, plan, tot, index);  // (a CTA that had prefixes has no own work: own_cta0)
   } else {
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // ------------------------------------ MMA issuer of chain `warp - kMmaWarp`
@@ -376,7 +391,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       uint32_t kn = 0, kp = 0, vn = 0, vp = 0;  // stage and phase of the coming K and V tile
       uint32_t items = 0, ns = 0, np = 0;       // items with tiles, S and P V of this chain
       bool ok = true;
-      if (elect_one()) while (walk.next(p, worker, im)) {
+      const bool issues = elect_one();
+      if (issues) while (walk.next(p, worker, im)) {
         if (!ok || im.n == 0) continue;
         const bool by_keys = im.rows <= 128;
         auto own = [&](int t) { return !by_keys || (t & 1) == c; };
@@ -431,6 +447,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
         if (!ok) report(p.dev_status, PA_DEVERR_TIMEOUT);
         items += any;
       }
+      if (issues && ns) {  // the CTA may not end before its products, taken or not
+        tc::mma_commit(&drained[c]);
+        (void)mbar_wait(&drained[c], 0);
+      }
     } else if (warp == kKWarp || warp == kVWarp) {
       // ---------------------------------------------------- K and V producers
       // Lane l < 4 NH loads one 16-row group x 64-column half of a tile; its
@@ -484,11 +504,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
           if (lane < NBOX && !manual) tc::tma_load_3d(dst, map, hf * 64, im.kvh, row, &full[st]);
         }
       }
-      if (!ok) {
-        if (lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
-        // copies still in flight land before the CTA gives up its memory
-        for (uint32_t i = n > (uint32_t)n_st ? n - n_st : 0; i < n; ++i)
-          (void)mbar_wait(&full[i % n_st], (i / n_st) & 1);
+      if (!ok && lane == 0) report(p.dev_status, PA_DEVERR_TIMEOUT);
+      // copies still in flight land before the CTA may end, taken or not: lane
+      // l waits for the last tile of stage l
+      if (lane < n_st && (uint32_t)lane < n) {
+        const uint32_t last = n - 1 - (n - 1 - lane) % n_st;
+        (void)mbar_wait(&full[lane], (last / n_st) & 1);
       }
     }
     __syncwarp();

@@ -53,6 +53,7 @@ SIGNATURES = {
     "pa_strerror": (ctypes.c_char_p, [_I]),
     "pa_last_cuda_error": (_I, []),
     "pa_set_merge_arrive_rounds": (_I, [_I]),
+    "pa_set_shared_waits": (_I, [_I]),
     "pa_choose_num_splits": (_I64, [_I64, _I64, _I64]),
     "pa_decode_workspace_size": (_I, [_I64, _I64, _I64, _I64, _I, _I64, _I64, _I64,
                                       ctypes.POINTER(_SZ)]),

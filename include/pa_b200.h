@@ -105,6 +105,12 @@ PA_API int pa_abi_version(void);
  * the default.  Process-wide; applies to launches made after the call.
  * Returns the previous value. */
 PA_API int pa_set_merge_arrive_rounds(int rounds);
+
+/* The same for the shared-prefix decode.  With `waits` 0 its tensor-core part
+ * gives up at the first scores it waits for, as it does after 1 s otherwise:
+ * the rows of prefixes done there are NaN (lse too) and PA_DEVERR_TIMEOUT is
+ * reported.  Any other value restores the wait; returns the previous one. */
+PA_API int pa_set_shared_waits(int waits);
 PA_API const char* pa_strerror(int status);
 /* cudaError_t of the most recent PA_ERR_CUDA on this thread (0 if none) */
 PA_API int pa_last_cuda_error(void);

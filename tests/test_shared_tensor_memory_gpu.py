@@ -86,3 +86,28 @@ def test_scales_of_zero(prefixes, D, dtype):
         check((q, kc, vc, bt, ctx, gs, pl), scale=scale)
     q[3, 5, 7], q[20, 31, 0] = float("inf"), float("nan")
     check((q, kc, vc, bt, ctx, gs, pl), scale=0.0)
+
+
+@pytest.mark.parametrize("prefix,members,D,dtype", [(300, 16, 128, torch.bfloat16), (20, 40, 64, torch.float16),
+                                                    (4000, 70, 128, torch.float16)])
+def test_waits_that_give_up(prefix, members, D, dtype):
+    """Every tensor-memory CTA stops at its first tile: its groups' rows are NaN, those of the other sequences
+    (a small group, one in none, an empty one) right; afterwards all of them are."""
+    groups = 20
+    starts = [g * members for g in range(groups + 1)]
+    prefixes = [prefix] * groups
+    n = starts[-1]
+    ctx = [prefix + b % 30 for b in range(n)] + [60, 50, 90, 0]
+    starts, prefixes = starts + [n + 2], prefixes + [40]
+    assert in_tensor_memory([(members, prefix)] * groups, 4, 8)
+    q, kc, vc, bt, ctx, gs, pl = make(members, 32, 8, D, dtype, 16, starts, prefixes, ctx)
+    want, mean_abs, want_lse = formula(q, kc, vc, bt, ctx, 0.1)
+    assert _lib.call("pa_set_shared_waits", 0) == 1
+    try:
+        out, lse, status = call(q, kc, vc, bt, ctx, gs, pl, 0.1)
+    finally:
+        assert _lib.call("pa_set_shared_waits", 1) == 0
+    assert status == _lib.PA_DEVERR_TIMEOUT
+    assert bool(out[:n].isnan().all()) and bool(lse[:n].isnan().all())
+    near(out[n:], lse[n:], want[n:], mean_abs[n:], want_lse[n:], dtype)
+    check((q, kc, vc, bt, ctx, gs, pl), scale=0.1)
