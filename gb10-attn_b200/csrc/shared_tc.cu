@@ -161,6 +161,23 @@ struct Walk {
   }
 };
 
+// What the softmax warps of a CTA that gave up do instead of their own work (a
+// CTA that had prefixes has none: own_cta0).  Every piece of its run becomes NaN,
+// done or not, and with it the output rows that have one; the merge's addresses
+// have to hold.  (Out of line: among the softmax warps' code it took registers
+// from the tiles, 128 sequences on 8k 60.7 us for 59.8.)
+__device__ __noinline__ void give_up(const Params& p, int64_t index) {
+  const Plan plan = plan_at(p, p.planned ? 0 : blockIdx.x);
+  const Totals tot = load_plan(plan.totals);
+  locate_rows(p, plan, tot, index);
+  const float nan = __int_as_float(0x7fc00000);
+  const int t = threadIdx.x;  // 128 x chain + row of the chain
+  Walk walk(p, plan, tot, blockIdx.x, t & 31);
+  TcItem im;
+  while (walk.next(p, blockIdx.x, im))
+    if ((im.rows <= 128 ? t & 127 : t) < im.rows) p.part_ml[im.prow + t] = make_float2(nan, nan);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_constant__ TcParams tp) {
   using C = TcCfg<D>;
@@ -349,17 +366,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
       }
     }
     if (!ok) {
-      // given up: every piece of the run is NaN, done or not, and so are the
-      // output rows that have one
       tc::tmem_wait_st();
       if (lane == 0) {
         atomicExch(abort_s, 1);
         report(p.dev_status, PA_DEVERR_TIMEOUT);
       }
-      const float nan = __int_as_float(0x7fc00000);
-      Walk again(p, plan, tot, worker, lane);
-      while (again.next(p, worker, im))
-        if ((im.rows <= 128 ? r : 128 * c + r) < im.rows) p.part_ml[im.prow + 128 * c + r] = make_float2(nan, nan);
     }
     // Both chains done: every product has been taken, and the shared memory is
     // free for the rings of the warps' own work
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const __grid_c
     if (*reinterpret_cast<volatile int32_t*>(abort_s) == 0)
       warp_work<T, D, C::STAGES>(p, plan, tot, smem_u32(smem) + warp * C::RING, own, index);
     else
-      locate_rows(p, plan, tot, index);  // (a CTA that had prefixes has no own work: own_cta0)
+      give_up(p, index);
   } else {
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // ------------------------------------ MMA issuer of chain `warp - kMmaWarp`
