@@ -384,10 +384,19 @@ class TorchBlockAllocator:
         q [B, n_head, head_dim], k, v [B, n_kv_head, head_dim] of the pool's
         type (fp16 or bf16), strided parts of one projection allowed;
         positions[b] is where sequence b's token goes (negative: idle),
-        context_lens[b] counts it.  Returns [B, n_head, head_dim]."""
+        context_lens[b] counts it.  Returns [B, n_head, head_dim].  What the
+        attention would refuse is refused before anything is appended."""
         from . import ops
         none = torch.empty(0, device=self.device)
         kc, vc = self.layer_kv(layer)
+        if kc.dtype not in (torch.float16, torch.bfloat16) or q.dtype != kc.dtype:
+            raise ValueError(f"layer_step_shared needs a float16 or bfloat16 pool and q of its type: "
+                             f"{kc.dtype} pool, {q.dtype} q")
+        if q.shape[1] % kc.shape[2]:
+            raise ValueError(f"{q.shape[1]} heads are no multiple of {kc.shape[2]} KV heads")
+        ng = prefix_lens.numel()
+        if (ng and group_starts.numel() != ng + 1) or context_lens.numel() < q.shape[0]:
+            raise ValueError("group_starts needs one entry more than prefix_lens, context_lens one a sequence")
         q = ops.qk_norm_rope_append(q, k, v, none if q_weight is None else q_weight,
                                     none if k_weight is None else k_weight, eps, cos_sin,
                                     interleaved, positions, none, kc, vc, block_tables, none, none)
