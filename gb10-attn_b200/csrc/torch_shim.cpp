@@ -772,7 +772,7 @@ std::tuple<torch::Tensor, torch::Tensor> paged_attention_shared(
   const int64_t B = qc.size(0), H = qc.size(1), D = qc.size(2);
   const int64_t NB = kc.size(0), BS = kc.size(1), HKV = kc.size(2), NG = pl.numel();
   TORCH_CHECK(kc.size(3) == D, op, ": k_cache head_dim must match q");
-  TORCH_CHECK(H % HKV == 0, "n_head must be divisible by n_kv_head");
+  TORCH_CHECK(HKV > 0 && H % HKV == 0, "n_head must be divisible by n_kv_head");
   TORCH_CHECK(bt.dim() == 2 && bt.size(0) >= B && ctx.numel() >= B,
               op, ": block_tables [B, MB] and context_lens [B] needed");
   TORCH_CHECK(NG == 0 || gs.numel() == NG + 1,
