@@ -189,7 +189,8 @@ class TorchBlockAllocator:
     def free(self, block_ids) -> None:
         """Give up one hold on each block; a block that forks share goes back
         to the pool with its last holder."""
-        for b in reversed(list(block_ids)):
+        ids = block_ids.tolist() if hasattr(block_ids, "tolist") else map(int, block_ids)
+        for b in reversed(list(ids)):
             left = self._shared.get(b, 0)
             if left == 0:
                 self._free.append(b)
