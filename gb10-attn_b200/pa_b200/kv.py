@@ -216,12 +216,16 @@ class TorchBlockAllocator:
         if rows and n > len(self._free):
             raise MemoryError(f"KV pool exhausted: need {n} blocks, {len(self._free)} free")
         shared = allocation.block_ids[:full]
+        last = [self._free.pop() for _ in range(n)] if rows else []
+        if last:
+            try:
+                self.copy_blocks([allocation.block_ids[full]] * n, last, [rows] * n)
+            except BaseException:
+                self._free.extend(reversed(last))
+                raise
         if n > 0:
             for b in shared:
                 self._shared[b] = self._shared.get(b, 0) + n
-        last = [self._free.pop() for _ in range(n)] if rows else []
-        if last:
-            self.copy_blocks([allocation.block_ids[full]] * n, last, [rows] * n)
         return [Allocation(shared + last[i:i + 1], t, list(allocation.token_ids[:t]))
                 for i in range(n)]
 

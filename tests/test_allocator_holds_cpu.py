@@ -24,3 +24,21 @@ def test_a_hold_is_given_up_whatever_form_the_ids_come_in(form):
     assert sorted(alloc._free) == list(range(16)) and all(type(b) is int for b in alloc._free) and not alloc._shared
     again = alloc.allocate(range(64))
     assert sorted(again.block_ids) == list(range(16))
+
+
+def test_a_fork_whose_copy_fails_changes_nothing(monkeypatch):
+    alloc = make()
+    a = alloc.allocate(range(10))
+    free = list(alloc._free)
+
+    def fail(*_):
+        raise RuntimeError("no copy")
+
+    monkeypatch.setattr(alloc, "copy_blocks", fail)
+    with pytest.raises(RuntimeError, match="no copy"):
+        alloc.fork(a, 3)
+    assert alloc._free == free and not alloc._shared
+    monkeypatch.setattr(alloc, "copy_blocks", lambda *_: None)
+    forks = alloc.fork(a, 3)
+    assert alloc.holders(a.block_ids[0]) == 4 and alloc.holders(a.block_ids[2]) == 1
+    assert len({f.block_ids[2] for f in forks} | {a.block_ids[2]}) == 4
