@@ -6,8 +6,8 @@
 //   out = (A_p + A_s) / (l_p + l_s),  A = sum_j e^{s_j - m} V_j, l = sum_j e^{s_j - m}
 // over the keys before and from P on, with one reference m, so the prefix can
 // be done for all members at once: their query heads of one KV head are the
-// rows of one product, and each K/V element of the prefix is read once a group
-// instead of once a sequence.
+// rows of products, and each K/V element of the prefix is read once for 16 rows
+// (by warps) or 256 (in tensor memory) instead of once for a sequence's.
 //
 // Two launches, the second a programmatic dependent of the first: the attention
 // and the merge of its partials.  Every CTA of the first makes the same plan in
@@ -32,6 +32,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Para
 }
 
 // All of the work by warps: pools that the tensor-memory part does not load.
+// Bound by the reads of a prefix for every 16 rows, out of the L2 mostly, and by
+// instruction latency.  128 sequences on 8k: 32 / 8 heads of 128 in pages of 8 166 us
+// (59 with the tensor memory, on pages of 16), 16 / 2 heads of 256 344, 32 / 8 of 32 66;
+// 64 on 2k, 12 / 12 heads of 64 in pages of 8, 22.
 template <int D> struct Cfg {
   static constexpr int STAGES = 4;
   static constexpr int RING = STAGES * (int)stage_bytes(D);
@@ -173,7 +177,11 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 // host
 // ---------------------------------------------------------------------------
 
-// Rows of a group from which its prefix may go to the tensor memory.
+// Rows of a group from which its prefix may go to the tensor memory.  Over 66
+// batches (listed beside kTcMinTiles) 17 takes 1.02 times as long and 65 1.01 times in the
+// mean: 17 up to 1.19 times (one group of 32 rows on 128 tokens 13.6 us, 16.1), 65
+// 0.82 times where many groups of 64 rows share 64 tokens (128 groups 164 us, 134),
+// 1.4 to 1.6 times where 4 or 8 groups of 48 or 64 rows share 8k (8 of 48: 84, 126).
 constexpr int kTcRows = 33;
 
 constexpr int64_t kAlign = 256;  // of the workspace's parts

@@ -147,7 +147,12 @@ __host__ __device__ constexpr int64_t plan_scratch(int64_t B, int64_t NG) {
 // four samples of 512 tokens, 29.9, 23.7, 22.0 for one sequence of 20k (its
 // pieces are more to merge).
 constexpr int kMinTiles = 3;
-constexpr int kTcMinTiles = 6;  // 64-key tiles per CTA below which the warps do all
+// 64-key tiles per CTA below which the warps do all.  Over 66 batches (2 to 1024
+// sequences of 8 to 512 rows a group, prefixes of 16 to 32768, head_dim 64 and 128) 2 and 4
+// take as long as 6 in the mean (2: 0.85 times for 64 on 2k with 32 / 8 heads, 1.06 at
+// most), 9 1.04 and 14 1.04 times: up to 2.2 times for 64 on 8k, which has 7 tiles a CTA
+// (41 us, 90), 0.85 times for 16 groups on 16 tokens.
+constexpr int kTcMinTiles = 6;
 // Tiles that a unit costs beside its own (swept: 1, 2, 4 of 16 keys and 2, 5, 8,
 // 14 of 64 keys give 76-82 us for 128 sequences on 8k, 56-60 for seven prompts,
 // each best at another; these are within 3 % of the best of both).
@@ -158,7 +163,8 @@ constexpr int kTcUnitCost = 6;
 // in percent of a tensor-memory tile of both chains (0.15 and 1.2 us).  Swept: 11,
 // 12, 13 with 75 to 85 give 260, 268, 245 us for 256 sequences on 32k (too few
 // CTAs for the own tokens are dear there), 63, 63, 65 for 128 on 8k, 50 for seven
-// prompts with any of them.
+// prompts with any of them.  Swept with head_dim 128 and four query heads a KV head;
+// others take the same.
 constexpr double kTileCost = 13, kTcSmallCost = 85;
 
 // Tiles that a unit of `keys` keys counts as.
@@ -492,8 +498,10 @@ __device__ __forceinline__ void locate_rows(const Params& p, const Plan& plan, c
 //   The keys of a tile are the N of S = Q K^T and the K of P V; the running
 // maximum and sum, the products' sums and O stay in fp32 registers.  P is rounded
 // to the pool's type for the second product (by 2^-9 or 2^-12 of a weight at most
-// and averaged over the keys: at the level of the output's own rounding); the
-// sum l is of the unrounded weights.
+// and averaged over the keys: at the level of the output's own rounding; in fp16 a
+// weight below 2^-14 of the piece's largest by up to 2^-25 of that, which
+// reaches the output's own rounding when some 2^13 keys weigh that little beside
+// one); the sum l is of the unrounded weights.
 //   HBM-bound on long runs on all SMs: 256 sequences' own 671 MB of 8 KV heads of 128
 // in 105 us (6.4 TB/s).  On fewer of them bound by the latency of its instructions,
 // 0.15 us a tile and SM, and some four such an item where units have a tile or two:

@@ -17,17 +17,20 @@
 // all SMs 1.05 PFLOP/s of S and P V, 63 % of the bf16 burst rate, 76 % of the
 // sustained one), while the CTAs with the sequences' own tokens are bound by
 // instruction latency (0.15 us a 16-key tile).  256 sequences of 32 / 8 heads of 128
-// behind 32768 tokens, with 256 to 1024 of their own: 246 us, some 88 CTAs with the
-// prefix and 60 with the rest.
+// behind 32768 tokens, with 256 to 1024 of their own: 275 to 297 us in steady calls,
+// by how far the power cap lowers the clock (246 from a cool start), some 88 CTAs
+// with the prefix and 60 with the rest.
 //   Tiles of 64 keys, not 128: two S of each chain then fit the tensor memory
 // beside both O, and S of the next tile is computed while a chain works on this
 // one (an MMA of N = 64 takes 48 cycles, of N = 128 64, but the pipe waits less).
 //   Precision: one 16-bit product each for S (Q and K as they are, products
-// exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be; the
-// sum l is of the unrounded weights).  The scale is applied to S in fp32.
-//   Every wait is bounded; on a timeout the CTA reports PA_DEVERR_TIMEOUT, stops
-// issuing work, makes NaN of the rows in its run, lets its copies and products
-// end and frees its tensor memory.
+// exact, fp32 sums) and P V (P rounded to 16 bits, as the output will be, in fp16
+// by up to 2^-25 where it is below 2^-14; the sum l is of the unrounded weights).
+// The scale is applied to S in fp32.
+//   Every wait is bounded; on a timeout the CTA reports PA_DEVERR_TIMEOUT to
+// callers that give a status word (the torch operators give none), stops issuing
+// work, makes NaN of the rows in its run, lets its copies and products end and
+// frees its tensor memory.
 #include <algorithm>
 #include <mutex>
 #include <vector>

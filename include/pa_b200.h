@@ -529,8 +529,9 @@ PA_API int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_
 
 /* Decode of sequences that share a prefix, an addition (the reference's decode
  * reads every sequence's whole context, kernels/paged_attn_v3.cu:192-261):
- * the result of pa_paged_attention_v3, with the keys and values of a group's
- * common prefix read once for all of its members.
+ * the attention of pa_paged_attention_v3 on 16-bit q and out, with the keys and
+ * values of a group's common prefix read once for 16 or 256 of its members'
+ * query heads (those of one KV head) instead of once for each member.
  *   Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1, and
  * its members have the same first prefix_lens[g] tokens: for those positions
  * their block-table rows lead to the same keys and values (the same pages, or
@@ -546,7 +547,8 @@ PA_API int pa_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_
  * that type for their product with V, out once at the end.  lse (nullable)
  * fp32 [num_seqs, num_heads].  A sequence with context_lens[b] <= 0 yields NaN
  * and lse -inf.  head_dim in {32, 64, 128, 256}; any block_size >= 1;
- * num_blocks * block_size * num_kv_heads < 2^32. */
+ * num_blocks * block_size * num_kv_heads < 2^32.  A wait that ran out (1 s)
+ * leaves NaN rows, lse too, and reports PA_DEVERR_TIMEOUT. */
 PA_API int pa_paged_attention_shared(
     void* out, float* lse, const void* q, int io_dtype, const void* k_cache, const void* v_cache,
     int kv_dtype, const int32_t* block_tables, const int32_t* context_lens,
